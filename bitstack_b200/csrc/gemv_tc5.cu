@@ -723,14 +723,13 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_tc5_kernel(const __grid_cons
         if (!landed) { GIVE_UP(8); ok = false; break; }
         const uint8_t* srow = S.sg + slot_s * kSlotBytes + tile_off;
         // two 16-byte pieces are in registers at a time; the slot may be refilled once all 256
-        // readers have taken their last piece
+        // readers have expanded their last piece
         uint4 v[2];
 #pragma unroll
         for (int pp = 0; pp < kPP; ++pp) {
           if ((pp & 1) == 0) {
             v[0] = *reinterpret_cast<const uint4*>(srow + (((piece0 + pp) ^ sw) << 4));
             v[1] = *reinterpret_cast<const uint4*>(srow + (((piece0 + pp + 1) ^ sw) << 4));
-            if (pp == kPP - 2) mbar_arrive(&S.sempty[slot_s]);
           }
           const int it = g * kPP + pp, slot = it & 1;
           TR_BEGIN(t2);
@@ -752,6 +751,10 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_tc5_kernel(const __grid_cons
           tmem_wait_st();
           tc_fence_before();
           if (!DBG_IS(2)) mbar_arrive(&S.afull[e][slot]);
+          // The last piece has been USED (its expansion is in tensor memory): only then may the slot be refilled.  An
+          // arrival directly behind the two loads does not wait for their data, and the refill two steps ahead was
+          // seen to overtake the second load.
+          if (pp == kPP - 1) mbar_arrive(&S.sempty[slot_s]);
         }
       }
       TR_ADD(0, t_prod);

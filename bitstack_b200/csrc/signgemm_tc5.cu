@@ -392,7 +392,6 @@ __global__ void __launch_bounds__(kThreads, 1) signgemm_tc5_kernel(const __grid_
       if (!mbar_wait(&stage_full[slot], (k / kStages) & 1, wait_ns)) { SG_GIVE_UP(34); ok = false; break; }
       const uint8_t* srow = s_stage + slot * kStageBytes + row * 64 + (((sub >> 1) ^ sw_s) << 4) + (sub & 1) * 8;
       const uint2 sw = *reinterpret_cast<const uint2*>(srow);
-      mbar_arrive(&stage_empty[slot]);
       const uint32_t w0 = __byte_perm(sw.x, 0, 0x0123), w1 = __byte_perm(sw.y, 0, 0x0123);   // column c -> bit 31 - c
       if (!mbar_wait(&p_full[g], use & 1, wait_ns)) { SG_GIVE_UP(35); ok = false; break; }
       tc_fence_after();
@@ -414,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) signgemm_tc5_kernel(const __grid_
         *reinterpret_cast<uint4*>(arow + ((c ^ sw_a) << 4)) = make_uint4(out[4 * c], out[4 * c + 1], out[4 * c + 2], out[4 * c + 3]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the stores must be visible to the MMA's reads
       mbar_arrive(&a_full[g]);
+      mbar_arrive(&stage_empty[slot]);          // behind the last use of the loaded sign words, not behind the load alone
     }
   } else {
     // ---- epilogue: a run's accumulator -> fp32 partial tile [tpad][128] ------------------------------------
