@@ -11,6 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("BITSTACK_B200_LIB") or os.path.join(_HERE, "libbitstack_b200.so")
 
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 ALGO_AUTO, ALGO_GENERAL, ALGO_REBUILD_GEMM, ALGO_GEMV_TC5, ALGO_SIGN_GEMM, ALGO_SIGN_GEMM_MMA = 0, 1, 3, 4, 5, 6
 
 
@@ -53,6 +54,14 @@ SIGNATURES = {
     "bsb_decode_attention_scratch_bytes": (C.c_int64, [_I32, _I32, _I32]),
     "bsb_greedy_step": (C.c_int, [_P, _I64, _I64, _I64, _P, _P, _P]),
     "bsb_silu_mul": (C.c_int, [_P, _P, _P, _P, _I64, _I32, _P]),
+    "bsb_page_tables": (C.c_int, [_P, _P, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "bsb_release_pages": (C.c_int, [_P, _P, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _P]),
+    "bsb_rope_paged_cache": (C.c_int, [_P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                                       _I32, _I32, _I32, _I32, _I32, _P]),
+    "bsb_paged_attention_scratch_bytes": (_I64, [_I32, _I32, _I32, _I32]),
+    "bsb_paged_decode_attention": (C.c_int, [_P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I32, _P, _P, _I64, _I64, _I64,
+                                             _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P]),
+    "bsb_sample_step": (C.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "bsb_peer_area_bytes": (_I64, [_I32, _I32, _I32]),
     "bsb_peer_alloc": (C.c_int, [_I64, C.POINTER(_P), _P]),
     "bsb_peer_open": (C.c_int, [_P, C.POINTER(_P)]),
@@ -92,6 +101,10 @@ class BitStackDeviceTimeout(BitStackLibraryError):
     """A time-bounded wait inside a kernel gave up; the outputs of that call are NaN."""
 
 
+class BitStackDeviceIndexError(BitStackLibraryError):
+    """A kernel met an index in device memory that points outside its tensor (a page, slot or position); it was not followed."""
+
+
 def check(rc: int, what: str):
     if rc != 0:
         msg = load().bsb_last_error().decode(errors="replace")
@@ -99,11 +112,14 @@ def check(rc: int, what: str):
             raise ValueError(f"{what}: {msg}")
         if rc == -5:
             raise BitStackDeviceTimeout(f"{what}: {msg}")
+        if rc == -6:
+            raise BitStackDeviceIndexError(f"{what}: {msg}")
         raise BitStackLibraryError(f"{what} failed ({rc}): {msg}")
 
 
 def check_device_status(clear: bool = True) -> None:
-    """Synchronises the current device and raises BitStackDeviceTimeout if any kernel of the library gave up a wait
-    since the status was last cleared.  Call it wherever the host waits for results anyway."""
+    """Synchronises the current device and raises BitStackDeviceTimeout if any kernel of the library gave up a wait,
+    BitStackDeviceIndexError if one met an index outside its tensor, since the status was last cleared.  Call it wherever
+    the host waits for results anyway."""
     code = C.c_int32(0)
     check(load().bsb_read_status(C.byref(code), 1 if clear else 0), "device status")

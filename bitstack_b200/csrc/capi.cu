@@ -354,6 +354,10 @@ int bsb_read_status(int32_t* code_out, int32_t clear) {
   BSB_CUDA(cudaDeviceSynchronize());   // every stream of the device: the word is shared by all of them
   BSB_CUDA(cudaMemcpy(code_out, word, 4, cudaMemcpyDeviceToHost));
   if (clear && *code_out != 0) BSB_CUDA(cudaMemset(word, 0, 4));
+  if (*code_out >= 61) {
+    set_error("a kernel met an index outside its tensor (code %d: 61 paged attention, 62 paged cache write, 63 token list, 64 page stack)", *code_out);
+    return BSB_EDATA;
+  }
   if (*code_out != 0) {
     set_error("a time-bounded wait gave up on the device (code %d): the outputs of that call are NaN", *code_out);
     return BSB_ETIMEOUT;
@@ -433,7 +437,7 @@ int bsb_linear_forward_host(const bsb_weight* w, const uint16_t* host_x, int64_t
   int32_t code = 0;
   BSB_CUDA(cudaMemcpyAsync(&code, device_status_word(), 4, cudaMemcpyDeviceToHost, s));
   BSB_CUDA(cudaStreamSynchronize(s));
-  if (code != 0) {   // the call's outputs are NaN; the word stays set until bsb_read_status() clears it
+  if (code != 0 && code < 61) {   // the call's outputs are NaN; the word stays set until bsb_read_status() clears it
     set_error("a time-bounded wait gave up on the device (code %d)", code);
     return BSB_ETIMEOUT;
   }

@@ -94,3 +94,170 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor, absmax: torch.Tensor = None) 
                                       None if absmax is None else absmax.data_ptr(), g2.shape[0], g2.shape[1], _s(gate))
     _lib.check(rc, "bsb_silu_mul")
     return out
+
+
+# ---------------------------------------------------------------------------------- serving over a paged cache
+_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
+def _need(t: torch.Tensor, name: str, dtype, shape, device, strided: bool = False) -> torch.Tensor:
+    """`t` as the kernels take it: CUDA tensor on `device`, given type and shape (None = any extent), contiguous, or with
+    `strided` only its last dimension."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on {device}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        raise ValueError(f"{name} must have shape {['any' if w is None else w for w in shape]}, got {list(t.shape)}")
+    if not (t.is_contiguous() or (strided and (t.shape[-1] <= 1 or t.stride(-1) == 1))):
+        raise ValueError(f"{name} must be contiguous" + (" in its last dimension" if strided else ""))
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _pages(k_pages, v_pages, dtype, kv_heads, head_dim, device):
+    """(num_pages, page_size, strides of a page) of a cache [num_pages, kv_heads, page_size, head_dim] whose pages are
+    contiguous; the pages themselves may lie apart (one allocation that interleaves K and V, or the layers)."""
+    _need(k_pages, "k_pages", dtype, (None, kv_heads, None, head_dim), device, strided=True)
+    _need(v_pages, "v_pages", dtype, tuple(k_pages.shape), device, strided=True)
+    n, _, ps, _ = k_pages.shape
+    if n < 1 or ps < 1:
+        raise ValueError("the page pool is empty")
+    inner = kv_heads * ps * head_dim
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not t[0].is_contiguous() or (n > 1 and t.stride(0) < inner):
+            raise ValueError(f"{name}: every page [kv_heads, page_size, head_dim] must be contiguous and apart from the next")
+    return n, ps, k_pages.stride(0) if n > 1 else inner, v_pages.stride(0) if n > 1 else inner
+
+
+def page_tables(lens, new_tokens, block_table, free_pages, free_count, page_size: int, max_tokens: int = 0, lens_out=None, free_count_out=None):
+    """One step of a paged cache's bookkeeping on the device: request b holds lens[b] tokens (int32 [batch]) and gets
+    new_tokens[b] more; pages it lacks are popped from the stack free_pages[:free_count] and entered in its row of
+    block_table (int32 [batch, width], updated in place).  lens and free_count (int32 [1]) are updated in place unless
+    lens_out / free_count_out receive the new values.  A request whose row is too narrow, or for which the stack runs out
+    (requests in order), is refused: it keeps its length.
+
+    Returns (slots, positions, offsets, last): slot and position of every new token, request after request, int64
+    [max_tokens], -1 for tokens of refused requests and behind the end; int32 [batch + 1] first token of every request;
+    int64 [batch] position of the request's last new token, -1 when it has none or was refused."""
+    dev = lens.device
+    batch = lens.shape[0] if lens.dim() == 1 else 0
+    _need(lens, "lens", torch.int32, (None,), dev)
+    _need(new_tokens, "new_tokens", torch.int32, (batch,), dev)
+    _need(block_table, "block_table", torch.int32, (batch, None), dev, strided=True)
+    _need(free_pages, "free_pages", torch.int32, (None,), dev)
+    _need(free_count, "free_count", torch.int32, (1,), dev)
+    lens_out = lens if lens_out is None else _need(lens_out, "lens_out", torch.int32, (batch,), dev)
+    free_count_out = free_count if free_count_out is None else _need(free_count_out, "free_count_out", torch.int32, (1,), dev)
+    if max_tokens < 0:
+        raise ValueError("max_tokens must not be negative")
+    with torch.cuda.device(dev):
+        lists = torch.empty(2, max_tokens, dtype=torch.int64, device=dev)
+        offsets = torch.empty(batch + 1, dtype=torch.int32, device=dev)
+        last = torch.empty(batch, dtype=torch.int64, device=dev)
+        rc = _lib.load().bsb_page_tables(lens.data_ptr(), new_tokens.data_ptr(), batch, block_table.data_ptr(), _row_stride(block_table),
+                                         block_table.shape[1], free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(),
+                                         int(page_size), int(max_tokens), lists[0].data_ptr(), lists[1].data_ptr(), offsets.data_ptr(),
+                                         last.data_ptr(), lens_out.data_ptr(), free_count_out.data_ptr(), _s(lens))
+    _lib.check(rc, "bsb_page_tables")
+    return lists[0], lists[1], offsets, last
+
+
+def release_pages(done, lens, block_table, free_pages, free_count, page_size: int) -> None:
+    """Requests with done[b] (bool [batch]) give their pages back to the stack, and their length becomes 0 (in place)."""
+    dev = lens.device
+    batch = lens.shape[0] if lens.dim() == 1 else 0
+    _need(lens, "lens", torch.int32, (None,), dev)
+    _need(done, "done", torch.bool, (batch,), dev)
+    _need(block_table, "block_table", torch.int32, (batch, None), dev, strided=True)
+    _need(free_pages, "free_pages", torch.int32, (None,), dev)
+    _need(free_count, "free_count", torch.int32, (1,), dev)
+    with torch.cuda.device(dev):
+        rc = _lib.load().bsb_release_pages(done.data_ptr(), lens.data_ptr(), batch, block_table.data_ptr(), _row_stride(block_table),
+                                           block_table.shape[1], free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(),
+                                           int(page_size), _s(lens))
+    _lib.check(rc, "bsb_release_pages")
+
+
+def _qkv(q, k, v, cos, sin, q_heads, kv_heads, head_dim):
+    dev, dtype = q.device, q.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"q must be fp16 or bf16, got {dtype}")
+    _need(q, "q", dtype, (None, q_heads * head_dim), dev, strided=True)
+    rows = q.shape[0]
+    _need(k, "k", dtype, (rows, kv_heads * head_dim), dev, strided=True)
+    _need(v, "v", dtype, (rows, kv_heads * head_dim), dev, strided=True)
+    _need(cos, "cos", dtype, (None, head_dim), dev)
+    _need(sin, "sin", dtype, tuple(cos.shape), dev)
+    return dev, dtype, rows
+
+
+def rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages, v_pages, q_heads, kv_heads, head_dim):
+    """Rotary embedding of a batch of tokens (a prompt, or several requests' tokens) at `positions` (int64 [tokens]); k and v
+    go to `slots` (int64 [tokens]) of k_pages / v_pages [num_pages, kv_heads, page_size, head_dim].  Returns the rotated q
+    [tokens, q_heads * head_dim].  Position -1: padding (its q row is 0, nothing is cached); slot -1: not cached."""
+    dev, dtype, rows = _qkv(q, k, v, cos, sin, q_heads, kv_heads, head_dim)
+    n, ps, ks, vs = _pages(k_pages, v_pages, dtype, kv_heads, head_dim, dev)
+    _need(positions, "positions", torch.int64, (rows,), dev)
+    _need(slots, "slots", torch.int64, (rows,), dev)
+    with torch.cuda.device(dev):
+        out = torch.empty(rows, q_heads * head_dim, dtype=dtype, device=dev)
+        rc = _lib.load().bsb_rope_paged_cache(q.data_ptr(), k.data_ptr(), v.data_ptr(), _row_stride(q), _row_stride(k), _row_stride(v),
+                                              cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(),
+                                              out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), n, ks, vs, rows, q_heads, kv_heads,
+                                              head_dim, ps, _DTYPES[dtype], _s(q))
+    _lib.check(rc, "bsb_rope_paged_cache")
+    return out
+
+
+def paged_decode_attention(q, k, v, cos, sin, positions, block_table, k_pages, v_pages, q_heads, kv_heads, head_dim):
+    """One new token per request at positions[b] (int64 [batch]; -1: idle row): rotary embedding of q and k, k and v written
+    into the request's page (block_table int32 [batch, width]), then grouped-query attention over positions 0 .. positions[b].
+    q, k, v: [batch, heads * head_dim], rows may be strided views; fp16 or bf16.  Returns [batch, q_heads * head_dim]."""
+    dev, dtype, rows = _qkv(q, k, v, cos, sin, q_heads, kv_heads, head_dim)
+    n, ps, ks, vs = _pages(k_pages, v_pages, dtype, kv_heads, head_dim, dev)
+    _need(positions, "positions", torch.int64, (rows,), dev)
+    _need(block_table, "block_table", torch.int32, (rows, None), dev, strided=True)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        out = torch.empty(rows, q_heads * head_dim, dtype=dtype, device=dev)
+        # scratch of this call alone: from the caching allocator, so that calls on other streams and other captured graphs have theirs
+        scratch = torch.empty(max(lib.bsb_paged_attention_scratch_bytes(rows, q_heads, kv_heads, head_dim), 16), dtype=torch.uint8, device=dev)
+        rc = lib.bsb_paged_decode_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), _row_stride(q), _row_stride(k), _row_stride(v),
+                                            cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), block_table.data_ptr(),
+                                            _row_stride(block_table), block_table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(), n, ks, vs,
+                                            out.data_ptr(), rows, q_heads, kv_heads, head_dim, ps, _DTYPES[dtype], scratch.data_ptr(),
+                                            scratch.numel(), _s(q))
+    _lib.check(rc, "bsb_paged_decode_attention")
+    return out
+
+
+def sample_step(logits, uniforms, tokens, temperature=None, top_k=None, top_p=None, min_p=None, pos=None, logprobs=None):
+    """tokens[b] (int64 [batch]) drawn from softmax(logits[b] / temperature[b]) with the given uniform number uniforms[b]
+    (fp32 [batch], in [0, 1)), after top-k, top-p and min-p (fp32 [batch], top_k int32 [batch]; None = off); then
+    pos[0] += 1 (skipped when pos is None).  logits: [batch, vocab] fp16, bf16 or fp32 with unit inner stride.
+    temperature 0: the first maximum, as `greedy_step`.  `logprobs` (fp32 [batch], optional) receives the log of the
+    token's probability among those kept."""
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
+    dev = logits.device
+    _need(logits, "logits", logits.dtype, (None, None), dev, strided=True)
+    batch, vocab = logits.shape
+    _need(uniforms, "uniforms", torch.float32, (batch,), dev)
+    _need(tokens, "tokens", torch.int64, (batch,), dev)
+    for t, name, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32), (logprobs, "logprobs", torch.float32)):
+        if t is not None:
+            _need(t, name, dtype, (batch,), dev)
+    if pos is not None:
+        _need(pos, "pos", torch.int64, (1,), dev)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with torch.cuda.device(dev):
+        rc = _lib.load().bsb_sample_step(logits.data_ptr(), batch, vocab, _row_stride(logits), _DTYPES[logits.dtype], uniforms.data_ptr(),
+                                         ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), tokens.data_ptr(), ptr(pos), ptr(logprobs),
+                                         _s(logits))
+    _lib.check(rc, "bsb_sample_step")
+    return tokens

@@ -35,6 +35,10 @@ extern "C" {
 #define BSB_EWORKSPACE (-3)/* scratch buffer missing or too small */
 #define BSB_ELIMIT (-4)    /* size beyond a documented maximum */
 #define BSB_ETIMEOUT (-5)  /* a time-bounded wait inside a kernel gave up; that call's outputs are NaN */
+#define BSB_EDATA (-6)     /* a kernel met an index in device memory that points outside its tensor (see bsb_read_status) */
+
+/* Element types of the entry points that serve more than fp16. */
+enum { BSB_F16 = 0, BSB_BF16 = 1, BSB_F32 = 2 };
 
 /* One stacked BitStack weight.  Strides are between consecutive blocks:
  * q_block_stride in bytes, u/vt_block_stride in fp16 elements.  `blocks` is the
@@ -180,6 +184,64 @@ int bsb_greedy_step(const uint16_t* logits, int64_t batch, int64_t vocab, int64_
 int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float* out_absmax, int64_t rows, int32_t n,
                  void* stream);
 
+/* ---- serving many requests: a paged key/value cache, and sampling (no counterpart in the reference, whose model calls
+ * are whole-sequence evaluations, bitstack/utils/model_utils.py:116-133) -------------------------------------------
+ * K and V live in pages: k_pages, v_pages [num_pages][kv_heads][page_size][head_dim], consecutive pages page_stride
+ * elements apart; row b of block_table (int32, rows table_stride apart, table_width entries) lists the pages of request b,
+ * position p of the request being row p % page_size of page block_table[b][p / page_size].  A SLOT is
+ * page * page_size + row.  fp16 or bf16 (`dtype`: q, k, v, the cos / sin tables [table_len][head_dim], pages and output
+ * alike), rows of q, k, v q_stride / k_stride / v_stride elements apart (multiples of 8), 16-byte aligned buffers.
+ * An index that points outside its tensor is never followed: see bsb_read_status, codes 61-64.
+ *
+ * bsb_page_tables: one step of all requests.  Request b holds lens[b] tokens and gets new_tokens[b] more (negative counts
+ *   are taken as 0).  Pages it lacks are popped from the stack free_pages[0 .. *free_count) (capacity entries), requests in
+ *   order, and entered in its row; entries of a row behind its pages are left as they are.  A request is REFUSED when its
+ *   row is too narrow, or when it needs pages and the stack holds fewer than it and the requests before it need together;
+ *   it keeps its length and its place in the token list.
+ *     offsets [batch + 1]       first token of every request in the list of all new tokens (request after request)
+ *     slots, positions [max_tokens]   of every new token; -1 for tokens of a refused request and behind the list's end
+ *     last [batch]              position of the request's last new token; -1 when it has none or was refused
+ *     lens_out, free_count_out  lengths and stack height afterwards; may be lens and free_count themselves
+ *   max_tokens == 0: no list is written (slots and positions may be NULL).  At most 8192 requests.
+ * bsb_release_pages: requests with done[b] != 0 give their pages back to the stack (in order) and get length 0.
+ * bsb_rope_paged_cache: rotary embedding ("rotate half") of `tokens` tokens: q_out [tokens][q_heads*head_dim] = rotated q;
+ *   rotated k and v go to the token's slot.  Slot -1: not cached; position -1: padding, its q_out row is 0 and nothing is
+ *   cached.  Slots of one call must differ.  head_dim % 16 == 0, <= 512.
+ * bsb_paged_decode_attention: one new token per request at positions[b] (its request then holds positions[b] + 1 tokens):
+ *   rotary embedding of q and k, k and v written into the page of that position, then softmax(q.K^T / sqrt(dim)).V over
+ *   positions 0 .. positions[b], grouped-query heads, fp32 softmax; out [batch][q_heads*dim].  positions[b] == -1: the row is
+ *   idle, its output is 0 and nothing is written.  Pages written by one request must not be read by another in the same call.
+ *   head_dim 64 or 128.  `scratch`: bsb_paged_attention_scratch_bytes, 16-byte aligned, contents arbitrary; calls that may
+ *   overlap need one each.
+ * bsb_sample_step: tokens[b] drawn from softmax(logits[b] / temperature[b]) cut by, in this order,
+ *   top_k (the k largest; <= 0: off), top_p (the smallest set of the largest whose weight reaches p of what top_k left;
+ *   >= 1: off), min_p (weight at least min_p of the largest; <= 0: off); ties go to the lowest index and the largest always
+ *   stays.  uniforms[b] in [0, 1): the token is the first in vocabulary order whose cumulative weight exceeds u times the
+ *   total.  temperature <= 0 (or NaN): the first maximum.  NaN logits count as -infinity; a row without a finite logit gives
+ *   token 0.  Each of temperature (1), top_k, top_p, min_p may be NULL (off).  logprobs[b] (may be NULL): log of the token's
+ *   probability among those kept.  *pos += 1 (pos may be NULL).  Same inputs, same token, bit for bit.  vocab <= 2^20. */
+int bsb_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t batch, int32_t* block_table, int64_t table_stride,
+                    int32_t table_width, const int32_t* free_pages, const int32_t* free_count, int32_t capacity, int32_t page_size,
+                    int64_t max_tokens, int64_t* slots, int64_t* positions, int32_t* offsets, int64_t* last, int32_t* lens_out,
+                    int32_t* free_count_out, void* stream);
+int bsb_release_pages(const uint8_t* done, int32_t* lens, int32_t batch, const int32_t* block_table, int64_t table_stride,
+                      int32_t table_width, int32_t* free_pages, int32_t* free_count, int32_t capacity, int32_t page_size, void* stream);
+int bsb_rope_paged_cache(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                         const void* cos_table, const void* sin_table, int64_t table_len, const int64_t* positions,
+                         const int64_t* slots, void* q_out, void* k_pages, void* v_pages, int64_t num_pages, int64_t k_page_stride,
+                         int64_t v_page_stride, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                         int32_t page_size, int32_t dtype, void* stream);
+int64_t bsb_paged_attention_scratch_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim);
+int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                               const void* cos_table, const void* sin_table, int64_t table_len, const int64_t* positions,
+                               const int32_t* block_table, int64_t table_stride, int32_t table_width, void* k_pages, void* v_pages,
+                               int64_t num_pages, int64_t k_page_stride, int64_t v_page_stride, void* out, int32_t batch,
+                               int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype, void* scratch,
+                               int64_t scratch_bytes, void* stream);
+int bsb_sample_step(const void* logits, int64_t batch, int64_t vocab, int64_t row_stride, int32_t dtype, const float* uniforms,
+                    const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens,
+                    int64_t* pos, float* logprobs, void* stream);
+
 /* ---- tensor parallelism: one-shot all-reduce over NVLink peer memory, fused with the add + RMSNorm that follows a
  * column-sharded projection.  No counterpart in the reference (single-device forward,
  * bitstack/modules/BitStackLinear.py:88-157).  One process per GPU; every rank owns an AREA of device memory that
@@ -235,7 +297,11 @@ int bsb_linear_forward_noalloc(const bsb_weight* w, const uint16_t* x, int64_t r
  *   bsb_read_status: synchronises the current device, copies the word to *code_out and, if `clear` is non-zero,
  *     resets it.  Returns BSB_OK when the word is 0, BSB_ETIMEOUT otherwise.  Codes: 1-8 decode kernel (1 Z' ring,
  *     2 Z' slab, 3/4 operand stage full/empty, 5/6 accumulator full/empty, 7/8 sign ring), 21-24 GEMM, 31-37 fused
- *     sign-GEMM, 51 peer all-reduce.
+ *     sign-GEMM, 51 peer all-reduce.  Codes from 61 on are not waits but bad indices in device memory, and give BSB_EDATA:
+ *     61 paged attention: a page outside the pool, or a position behind the table row or the cos / sin tables (the
+ *     request's output is NaN); 62 bsb_rope_paged_cache: a slot outside the pool (not written) or a position behind the
+ *     cos / sin tables (q row NaN, not cached); 63 bsb_page_tables: more new tokens than max_tokens (the list is cut);
+ *     64 bsb_release_pages: more pages than the stack has room for (the rest are lost).
  *     Call it wherever the host synchronises anyway (bsb_linear_forward_host does).
  *   bsb_set_wait_limit_ms: the time limit of every such wait (default 200 ms), for kernels launched afterwards. */
 int bsb_read_status(int32_t* code_out, int32_t clear);
