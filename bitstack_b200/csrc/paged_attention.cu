@@ -1,5 +1,19 @@
 // One new token per request over a paged key/value cache: rotary embedding of q and k, k and v written into the request's
 // page, softmax(q K^T / sqrt(D)) V over the request's pages.
+//
+// Bound by reading K and V once (4 flops per byte and head of a group; the floor is their bytes at copy bandwidth).
+//  * Work split: a request's length is cut into tiles of 64 positions; the tiles of all (request, kv head) pairs form one
+//    sequence, of which every CTA takes the same number.  Lengths are only known on the device, so every CTA finds its place
+//    by a prefix sum over the requests.  A pair that several CTAs share leaves partial results (maximum, sum, unnormalised
+//    output), which a second kernel joins in CTA order: no atomics, no state between calls, the same bits every time.
+//  * A CTA is four warps, and a warp is on its own: it streams its 16 positions of every tile through a ring of its own in
+//    shared memory (16-byte cp.async, rows looked up page by page, so a page may end anywhere) and needs no barrier with the
+//    others until the pair ends.  Rows behind the last position are filled with zeros, whatever the page holds there.
+//  * All query heads of a group (up to 16, the M of mma.sync m16n8k16) share the K and V that were read; scores and output are
+//    accumulated in fp32, the weights are rounded to the cache's type for the second product (half a step of relative error
+//    each, as q is rounded after its rotation), and one pass keeps the running maximum and sum.
+//  * The new position's K and V come from the projection's output: turned, stored to the page and to the ring by the warp
+//    that meets the position, so nothing is read back.
 #include <climits>
 #include <math.h>
 
@@ -9,99 +23,467 @@
 namespace bsb {
 namespace {
 
-// One CTA per (query head, request); a warp takes every fourth position, its lanes share the row.  One pass with the
-// running maximum and sum of the softmax; the four warps are joined in shared memory.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-                                                              int64_t q_stride, int64_t k_stride, int64_t v_stride, const T* __restrict__ cos_t,
-                                                              const T* __restrict__ sin_t, int64_t table_len, const int64_t* __restrict__ positions,
-                                                              const int32_t* __restrict__ table, int64_t table_stride, int width, T* __restrict__ k_pages,
-                                                              T* __restrict__ v_pages, int64_t num_pages, int64_t k_page_stride, int64_t v_page_stride,
-                                                              T* __restrict__ out, int Hq, int Hkv, int page_size, float scale, int* __restrict__ status) {
-  constexpr int E = D / 32;
-  __shared__ float s_q[D], s_k[D], s_o[4][D], s_m[4], s_l[4];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 16 * kWarps;       // positions of a tile
+constexpr int kRows = 16;                // query heads of one pass (the M of the MMA)
+constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix sums stay in shared memory
+constexpr int64_t kWholePositions = 512; // requests that cannot be longer than this get one CTA per (request, kv head): no join
+
+template <int D> struct Shape;
+template <> struct Shape<128> { static constexpr int stages = 3, ctas = 2; };
+template <> struct Shape<64> { static constexpr int stages = 4, ctas = 3; };
+
+struct AttnParams {
+  const void *q, *k, *v, *cos_t, *sin_t;
+  void *k_pages, *v_pages, *out;
+  int64_t q_stride, k_stride, v_stride, k_page_stride, v_page_stride, table_len, num_pages, table_stride;
+  const int64_t* positions;
+  const int32_t* table;
+  int64_t most;                          // positions that a table row can hold
+  int batch, Hq, Hkv, group, chunks, rows_kept, page_size;
+  float scale_log2;
+  float* part;                           // [CTA][2]: 16 maxima, 16 sums, rows_kept x D outputs (every part 16-byte aligned)
+  int4* plan;                            // [CTA]: first output row, heads, last CTA of the shared pair that begins in this CTA; heads == 0: none
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool keep) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(keep ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const typename Pair<T>::type p = Pair<T>::make(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// tokens a request holds after this step; -1: its position is behind its table row or the cos / sin tables
+__device__ __forceinline__ int64_t length_of(const AttnParams& P, int b) {
+  const int64_t pos = P.positions[b];
+  if (pos < 0) return 0;
+  return pos < P.most && pos < P.table_len ? pos + 1 : -1;
+}
+__device__ __forceinline__ int64_t tiles_of(int64_t n) { return n <= 0 ? 1 : (n + kTile - 1) / kTile; }   // idle rows too have an output
+
+// dynamic shared memory: [warp][stage][K 16 rows, V 16 rows], q [16 rows], maxima and sums [2][warp][16], prefix sums [batch + 1]
+template <int D> constexpr int ring_bytes() { return kWarps * Shape<D>::stages * 2 * 16 * D * 2; }
+template <int D> constexpr int fixed_bytes() { return ring_bytes<D>() + kRows * D * 2 + 2 * kWarps * kRows * 4; }
+
+template <typename T, int D, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kernel(const __grid_constant__ AttnParams P) {
+  constexpr int kStages = Shape<D>::stages;
+  constexpr int kChunks = D / 8;                 // 16-byte pieces of a row
+  constexpr int kStep = 32 / kChunks;            // rows that one warp-wide copy covers
+  constexpr int kHalf = 16 * D * 2;              // bytes of the K (or V) rows of a stage
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* s_q = smem + ring_bytes<D>();
+  float* s_m = reinterpret_cast<float*>(s_q + kRows * D * 2);
+  float* s_l = s_m + kWarps * kRows;
+  int64_t* s_before = reinterpret_cast<int64_t*>(s_l + kWarps * kRows);
+  __shared__ int64_t s_sum[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pairs = P.Hkv * P.chunks;            // (kv head, chunk of its query heads)
   pdl_enter();
-  const int64_t pos = positions[b];
-  T* o = out + ((int64_t)b * Hq + h) * D;
+
+  // ---- this CTA's share of the tiles ------------------------------------------------------------------------------
+  int64_t first, end, share = 0;
+  int b, pair;
+  int64_t t0 = 0;
+  if (WHOLE) {
+    b = blockIdx.x / pairs;
+    pair = blockIdx.x - b * pairs;
+    first = 0;
+    end = tiles_of(length_of(P, b));
+  } else {
+    const int each = (P.batch + kThreads - 1) / kThreads;
+    const int lo = min(tid * each, P.batch), hi = min(lo + each, P.batch);
+    int64_t mine = 0;
+    for (int i = lo; i < hi; ++i) mine += tiles_of(length_of(P, i));
+    int64_t upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += s_sum[w];
+    int64_t run = upto - mine;
+    for (int i = lo; i < hi; ++i) {
+      s_before[i] = run;
+      run += tiles_of(length_of(P, i));
+    }
+    if (tid == kThreads - 1) s_before[P.batch] = upto;
+    __syncthreads();
+    const int64_t total = s_before[P.batch] * pairs;
+    share = (total + gridDim.x - 1) / gridDim.x;
+    first = min(blockIdx.x * share, total);
+    end = min(first + share, total);
+    if (tid == 0) P.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (first == end) return;
+    int l = 0, h = P.batch - 1;                  // the request of tile `first`
+    while (l < h) {
+      const int mid = (l + h + 1) >> 1;
+      if (s_before[mid] * pairs <= first) l = mid;
+      else h = mid - 1;
+    }
+    b = l;
+    const int64_t in = first - s_before[b] * pairs, tiles = s_before[b + 1] - s_before[b];
+    pair = (int)(in / tiles);
+    t0 = in - pair * tiles;
+  }
+
+  uint8_t* ring = smem + warp * (kStages * 2 * kHalf);
+  const uint32_t ring_at = smem_u32(ring);
+  const int gid = lane >> 2, t4 = lane & 3;
   const float nan = __int_as_float(0x7FC00000);
-  if (pos < 0) {
-    if (tid < D) o[tid] = Pair<T>::one(0.f);
-    return;
-  }
-  if (pos >= table_len || pos >= (int64_t)width * page_size) {
-    if (tid < D) o[tid] = Pair<T>::one(nan);
-    if (tid == 0) atomicCAS(status, 0, 61);
-    return;
-  }
-  const int g = Hq / Hkv, hk = h / g;
-  const T* qs = q + b * q_stride + (int64_t)h * D;
-  const T* ks = k + b * k_stride + (int64_t)hk * D;
-  const T* vs = v + b * v_stride + (int64_t)hk * D;
-  const int32_t* pages = table + b * table_stride;
-  for (int i = tid; i < D / 2; i += 128) {
-    const float c0 = to_f(cos_t[pos * D + i]), c1 = to_f(cos_t[pos * D + i + D / 2]);
-    const float s0 = to_f(sin_t[pos * D + i]), s1 = to_f(sin_t[pos * D + i + D / 2]);
-    float x0 = to_f(qs[i]), x1 = to_f(qs[i + D / 2]);
-    s_q[i] = (x0 * c0 - x1 * s0) * scale;
-    s_q[i + D / 2] = (x1 * c1 + x0 * s1) * scale;
-    x0 = to_f(ks[i]);
-    x1 = to_f(ks[i + D / 2]);
-    s_k[i] = to_f(Pair<T>::one(x0 * c0 - x1 * s0));
-    s_k[i + D / 2] = to_f(Pair<T>::one(x1 * c1 + x0 * s1));
-  }
-  __syncthreads();
-  bool bad = false;
-  const int page_new = pages[pos / page_size];
-  if (page_new < 0 || page_new >= num_pages) bad = true;
-  else if (h % g == 0 && tid < D) {
-    k_pages[page_new * k_page_stride + ((int64_t)hk * page_size + pos % page_size) * D + tid] = Pair<T>::one(s_k[tid]);
-    v_pages[page_new * v_page_stride + ((int64_t)hk * page_size + pos % page_size) * D + tid] = vs[tid];
-  }
-  float m = -INFINITY, l = 0.f, acc[E];
+
+  for (int64_t at = first; at < end;) {
+    const int64_t len = length_of(P, b);
+    const int64_t n = max(len, (int64_t)0);
+    const int64_t tiles = tiles_of(len);
+    const int nt = (int)min(tiles - t0, end - at);                 // tiles of this pair that are this CTA's
+    const int hk = pair / P.chunks, head0 = hk * P.group + (pair - hk * P.chunks) * kRows;
+    const int heads = min(kRows, (hk + 1) * P.group - head0);
+    const int32_t* pages = P.table + (int64_t)b * P.table_stride;
+    bool bad = len < 0;
+
+    // ---- q: turned, rounded to the type, rows behind the group zero ------------------------------------------------
+    for (int it = tid; it < kRows * (D / 16); it += kThreads) {
+      const int r = it / (D / 16), c = it - r * (D / 16);
+      float x0[8], x1[8];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int64_t p = warp; p <= pos; p += 4) {
-    float kv[E], vv[E];
-    if (p == pos) {
+      for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
+      if (r < heads && n > 0) {
+        const T* src = (const T*)P.q + b * P.q_stride + (int64_t)(head0 + r) * D + c * 8;
+        float c0[8], c1[8], s0[8], s1[8];
+        load8(src, x0);
+        load8(src + D / 2, x1);
+        load8((const T*)P.cos_t + (n - 1) * D + c * 8, c0);
+        load8((const T*)P.cos_t + (n - 1) * D + c * 8 + D / 2, c1);
+        load8((const T*)P.sin_t + (n - 1) * D + c * 8, s0);
+        load8((const T*)P.sin_t + (n - 1) * D + c * 8 + D / 2, s1);
 #pragma unroll
-      for (int e = 0; e < E; ++e) { kv[e] = s_k[lane + 32 * e]; vv[e] = to_f(vs[lane + 32 * e]); }
-    } else {
-      const int page = pages[p / page_size];
-      if (page < 0 || page >= num_pages) { bad = true; break; }
-      const int64_t row = ((int64_t)hk * page_size + p % page_size) * D;
+        for (int e = 0; e < 8; ++e) {
+          const float a = x0[e], d = x1[e];
+          x0[e] = a * c0[e] - d * s0[e];
+          x1[e] = d * c1[e] + a * s1[e];
+        }
+      }
+      *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((c ^ (r & 7)) << 4)) = pack8<T>(x0);
+      *reinterpret_cast<uint4*>(s_q + r * D * 2 + (((c + D / 16) ^ (r & 7)) << 4)) = pack8<T>(x1);
+    }
+    __syncthreads();
+    uint32_t qf[D / 16][4];
+    {
+      const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        kv[e] = to_f(k_pages[page * k_page_stride + row + lane + 32 * e]);
-        vv[e] = to_f(v_pages[page * v_page_stride + row + lane + 32 * e]);
+      for (int ks = 0; ks < D / 16; ++ks) ldsm4(smem_u32(s_q) + r * D * 2 + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4), qf[ks]);
+    }
+
+    // ---- the ring: lane r (and r + 16) knows where row r of the tile to come lies ------------------------------------
+    const int64_t base0 = t0 * kTile + warp * 16;
+    int page_next = 0;
+    auto look_up = [&](int i) {                   // page of this lane's row in tile i of the share; loaded one tile ahead of its use
+      const int64_t p = base0 + (int64_t)i * kTile + (lane & 15);
+      page_next = i < nt && p < n ? pages[p / P.page_size] : 0;
+    };
+    auto issue = [&](int i) {
+      if (i < nt) {
+        const int64_t p = base0 + (int64_t)i * kTile + (lane & 15);
+        const int page = page_next;
+        const bool valid = p < n;
+        const bool found = valid && page >= 0 && page < P.num_pages;
+        if (valid && !found) bad = true;
+        const int in_page = (int)(p % P.page_size);
+        const bool fresh = p == n - 1;
+        const int code = fresh ? -2 : found ? page : -1;   // -2: written below, -1: zeros
+        look_up(i + 1);
+        const uint32_t dst = ring_at + (i % kStages) * (2 * kHalf);
+#pragma unroll
+        for (int j = 0; j < 16; j += kStep) {
+          const int r = j + lane / kChunks, c = lane % kChunks;
+          const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
+          const bool keep = pg >= 0;
+          const int64_t off = ((int64_t)hk * P.page_size + rw) * D + c * 8;
+          const uint32_t d = dst + r * D * 2 + ((c ^ (r & 7)) << 4);
+          const T* ks = (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0);
+          const T* vs = (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0);
+          if (pg != -2) {
+            cp_async16(d, ks, keep);
+            cp_async16(d + kHalf, vs, keep);
+          }
+        }
+        // the new position: in the last tile only
+        const uint32_t who = __ballot_sync(0xFFFFFFFFu, fresh && lane < 16);
+        if (who != 0) {
+          const int r = __ffs(who) - 1;
+          const int pg = __shfl_sync(0xFFFFFFFFu, found ? page : -1, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
+          const bool write = pg >= 0 && pair == hk * P.chunks;
+          const int64_t off = ((int64_t)hk * P.page_size + rw) * D;
+          T* kd = (T*)P.k_pages + (write ? pg * P.k_page_stride + off : 0);
+          T* vd = (T*)P.v_pages + (write ? pg * P.v_page_stride + off : 0);
+          uint8_t* row = ring + (i % kStages) * (2 * kHalf) + r * D * 2;
+          if (lane < D / 16) {
+            const T* src = (const T*)P.k + b * P.k_stride + (int64_t)hk * D + lane * 8;
+            float x0[8], x1[8], c0[8], c1[8], s0[8], s1[8];
+            load8(src, x0);
+            load8(src + D / 2, x1);
+            load8((const T*)P.cos_t + (n - 1) * D + lane * 8, c0);
+            load8((const T*)P.cos_t + (n - 1) * D + lane * 8 + D / 2, c1);
+            load8((const T*)P.sin_t + (n - 1) * D + lane * 8, s0);
+            load8((const T*)P.sin_t + (n - 1) * D + lane * 8 + D / 2, s1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float a = x0[e], d = x1[e];
+              x0[e] = a * c0[e] - d * s0[e];
+              x1[e] = d * c1[e] + a * s1[e];
+            }
+            const uint4 lo = pack8<T>(x0), hi = pack8<T>(x1);
+            *reinterpret_cast<uint4*>(row + ((lane ^ (r & 7)) << 4)) = lo;
+            *reinterpret_cast<uint4*>(row + (((lane + D / 16) ^ (r & 7)) << 4)) = hi;
+            if (write) {
+              *reinterpret_cast<uint4*>(kd + lane * 8) = lo;
+              *reinterpret_cast<uint4*>(kd + lane * 8 + D / 2) = hi;
+            }
+          } else if (lane >= 16 && lane < 16 + D / 8) {
+            const int c = lane - 16;
+            const uint4 x = *reinterpret_cast<const uint4*>((const T*)P.v + b * P.v_stride + (int64_t)hk * D + c * 8);
+            *reinterpret_cast<uint4*>(row + kHalf + ((c ^ (r & 7)) << 4)) = x;
+            if (write) *reinterpret_cast<uint4*>(vd + c * 8) = x;
+          }
+        }
+      }
+      cp_async_commit();
+    };
+
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[D / 8][4];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+
+    look_up(0);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) issue(i);
+    for (int i = 0; i < nt; ++i) {
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const int64_t base = base0 + (int64_t)i * kTile;
+      if (base < n) {
+        const uint32_t kt = ring_at + (i % kStages) * (2 * kHalf), vt = kt + kHalf;
+        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        {
+          const int r = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t kf[4];
+            ldsm4(kt + r * D * 2 + (((2 * ks + ((lane >> 3) & 1)) ^ (r & 7)) << 4), kf);
+            mma16816<T>(s[0], qf[ks], kf[0], kf[1]);
+            mma16816<T>(s[1], qf[ks], kf[2], kf[3]);
+          }
+        }
+        const int left = (int)min(n - base, (int64_t)16);   // positions of these 16 that exist
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool in = h * 8 + t4 * 2 + e < left;
+            s[h][e] = in ? s[h][e] * P.scale_log2 : -INFINITY;
+            s[h][e + 2] = in ? s[h][e + 2] * P.scale_log2 : -INFINITY;
+            x0 = fmaxf(x0, s[h][e]);
+            x1 = fmaxf(x1, s[h][e + 2]);
+          }
+#pragma unroll
+        for (int w = 1; w < 4; w <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, w));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, w));
+        }
+        x0 = fmaxf(x0, m0);                       // finite: at least one position exists
+        x1 = fmaxf(x1, m1);
+        if (__any_sync(0xFFFFFFFFu, x0 > m0 || x1 > m1)) {
+          const float f0 = fast_exp2(m0 - x0), f1 = fast_exp2(m1 - x1);
+          l0 *= f0;
+          l1 *= f1;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            o[j][0] *= f0;
+            o[j][1] *= f0;
+            o[j][2] *= f1;
+            o[j][3] *= f1;
+          }
+          m0 = x0;
+          m1 = x1;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[h][e] = fast_exp2(s[h][e] - m0);
+            s[h][e + 2] = fast_exp2(s[h][e + 2] - m1);
+            l0 += s[h][e];
+            l1 += s[h][e + 2];
+          }
+        const uint32_t pf[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+        {
+          const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+          for (int j = 0; j < D / 8; j += 2) {
+            uint32_t vf[4];
+            ldsm4_t(vt + r * D * 2 + (((j + (lane >> 4)) ^ (r & 7)) << 4), vf);
+            mma16816<T>(o[j], pf, vf[0], vf[1]);
+            mma16816<T>(o[j + 1], pf, vf[2], vf[3]);
+          }
+        }
+      }
+      __syncwarp();                               // every lane has read the stage before it is filled again
+      issue(i + kStages);
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    if (bad) atomicCAS(P.status, 0, 61);
+    bad = __syncthreads_or(bad);                  // (also: q may be overwritten from here on)
+
+    // ---- the four warps' results, joined ------------------------------------------------------------------------------
+#pragma unroll
+    for (int w = 1; w < 4; w <<= 1) {
+      l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, w);
+      l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, w);
+    }
+    if (t4 == 0) {
+      s_m[warp * kRows + gid] = m0;
+      s_m[warp * kRows + gid + 8] = m1;
+      s_l[warp * kRows + gid] = l0;
+      s_l[warp * kRows + gid + 8] = l1;
+    }
+    float* mine = reinterpret_cast<float*>(ring);   // [16][D] fp32: no more than a ring of two stages
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      const int col = (j * 8 + t4 * 2) ^ (gid * 8 & (D - 1));   // rows shifted against one another: no bank conflicts
+      if (gid < heads) *reinterpret_cast<float2*>(mine + gid * D + col) = make_float2(o[j][0], o[j][1]);
+      if (gid + 8 < heads) *reinterpret_cast<float2*>(mine + (gid + 8) * D + col) = make_float2(o[j][2], o[j][3]);
+    }
+    __syncthreads();
+    const bool begins = t0 == 0, ends = t0 + nt == tiles;
+    const int slot_floats = 2 * kRows + P.rows_kept * D;
+    float* part = WHOLE ? nullptr : P.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * slot_floats;
+    const int64_t out_row = (int64_t)b * P.Hq + head0;
+    for (int it = tid; it < heads * (D / 4); it += kThreads) {
+      const int r = it / (D / 4), c = (it - r * (D / 4)) * 4;
+      float m = s_m[r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w * kRows + r]);
+      float l = 0.f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = s_m[w * kRows + r], f = mw == -INFINITY ? 0.f : fast_exp2(mw - m);
+        const float4 x = *reinterpret_cast<const float4*>(smem + w * (kStages * 2 * kHalf) + (r * D + (c ^ ((r & 7) * 8 & (D - 1)))) * 4);
+        l += s_l[w * kRows + r] * f;
+        a.x += x.x * f;
+        a.y += x.y * f;
+        a.z += x.z * f;
+        a.w += x.w * f;
+      }
+      if (bad) l = nan;
+      if (begins && ends) {
+        const float inv = n > 0 || bad ? 1.f / l : 0.f;            // idle: zeros
+        uint2 packed;
+        packed.x = pack2<T>(a.x * inv, a.y * inv);
+        packed.y = pack2<T>(a.z * inv, a.w * inv);
+        *reinterpret_cast<uint2*>((T*)P.out + (out_row + r) * D + c) = packed;
+      } else {
+        *reinterpret_cast<float4*>(part + 2 * kRows + r * D + c) = a;
+        if (c == 0) {
+          part[r] = m;
+          part[kRows + r] = l;
+        }
       }
     }
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(kv[e], s_q[lane + 32 * e], s);
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, w);
-    const float mn = fmaxf(m, s), f = __expf(m - mn), e1 = __expf(s - mn);
-    l = l * f + e1;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + e1 * vv[e];
-    m = mn;
-  }
-  if (bad) { l = nan; if (lane == 0) atomicCAS(status, 0, 61); }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = acc[e];
-  __syncthreads();
-  if (tid < D) {
-    float mm = -INFINITY, ll = 0.f, oo = 0.f;
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, s_m[w]);
-    for (int w = 0; w < 4; ++w) {
-      const float f = s_m[w] == -INFINITY ? 0.f : __expf(s_m[w] - mm);
-      ll += s_l[w] * f;
-      oo += s_o[w][tid] * f;
-      if (s_l[w] != s_l[w]) ll = nan;
+    if (!WHOLE && begins && !ends && tid == 0) {   // this CTA's last pair: the CTAs behind hold the rest of it
+      const int64_t pair_end = at + tiles;
+      P.plan[blockIdx.x] = make_int4((int)out_row, heads, (int)((pair_end - 1) / share), 0);
     }
-    o[tid] = Pair<T>::one(oo / ll);
+    __syncthreads();                              // the ring is free again
+    at += nt;
+    t0 = 0;
+    if (++pair == pairs) {
+      pair = 0;
+      ++b;
+    }
   }
+}
+
+// shared pairs: CTA c joins the pair that began in c's share and ends in that of plan[c].z
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_constant__ AttnParams P) {
+  pdl_enter();
+  const int c0 = blockIdx.x;
+  const int4 plan = P.plan[c0];
+  const int slot = 2 * kRows + P.rows_kept * D;
+  for (int it = threadIdx.x; it < plan.y * (D / 2); it += blockDim.x) {
+    const int r = it / (D / 2), c = (it - r * (D / 2)) * 2;
+    float m = P.part[((int64_t)c0 * 2 + 1) * slot + r];
+    for (int i = c0 + 1; i <= plan.z; ++i) m = fmaxf(m, P.part[(int64_t)i * 2 * slot + r]);
+    float l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll 4
+    for (int i = c0; i <= plan.z; ++i) {
+      const float* part = P.part + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * slot;
+      const float f = fast_exp2(part[r] - m);
+      const float2 o = *reinterpret_cast<const float2*>(part + 2 * kRows + r * D + c);
+      l += part[kRows + r] * f;
+      x += o.x * f;
+      y += o.y * f;
+    }
+    const float inv = 1.f / l;
+    *reinterpret_cast<uint32_t*>((T*)P.out + ((int64_t)plan.x + r) * D + c) = pack2<T>(x * inv, y * inv);
+  }
+}
+
+template <typename T, int D>
+int launch_paged_attention(AttnParams P, cudaStream_t s) {
+  const int pairs = P.Hkv * P.chunks;
+  const bool whole = P.most <= kWholePositions;
+  const int grid = whole ? P.batch * pairs : sm_count() * Shape<D>::ctas;
+  const size_t smem = fixed_bytes<D>() + (whole ? 0 : (size_t)(P.batch + 1) * 8);
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  BSB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed_bytes<D>() + (kMaxBatch + 1) * 8));
+    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed_bytes<D>()));
+    attr_set[dev] = true;
+  }
+  if (whole) {
+    BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, true>, dim3(grid), dim3(kThreads), smem, s, P));
+    return check_launch("paged_attention_kernel");
+  }
+  BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, false>, dim3(grid), dim3(kThreads), smem, s, P));
+  if (int rc = check_launch("paged_attention_kernel")) return rc;
+  BSB_CUDA(launch_pdl(paged_attention_join_kernel<T, D>, dim3(grid), dim3(256), 0, s, P));
+  return check_launch("paged_attention_join_kernel");
 }
 
 }  // namespace
@@ -113,7 +495,8 @@ extern "C" {
 
 int64_t bsb_paged_attention_scratch_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (batch < 0 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || q_heads % kv_heads != 0) return -1;
-  return 0;
+  const int rows = q_heads / kv_heads < kRows ? q_heads / kv_heads : kRows;
+  return (int64_t)sm_count() * 3 * (16 + 2 * (2 * kRows + (int64_t)rows * head_dim) * 4);
 }
 
 int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -135,24 +518,54 @@ int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int6
   BSB_CHECK_ARG((q_stride | k_stride | v_stride | k_page_stride | v_page_stride) % 8 == 0, "strides must be multiples of 8 elements");
   BSB_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos_table | (uintptr_t)sin_table | (uintptr_t)out |
                  (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0, "buffers must be 16-byte aligned");
-  if (batch > 65535) {
-    set_error("paged attention: at most 65535 requests per call (got %d)", batch);
-    return BSB_ELIMIT;
+  BSB_CHECK_ARG((int64_t)batch * q_heads <= INT_MAX, "batch * q_heads too large");
+  const int64_t need = bsb_paged_attention_scratch_bytes(batch, q_heads, kv_heads, head_dim);
+  BSB_CHECK_ARG(scratch != nullptr && (uintptr_t)scratch % 16 == 0, "scratch is NULL or not 16-byte aligned");
+  if (scratch_bytes < need) {
+    set_error("scratch of %lld bytes needed, %lld given", (long long)need, (long long)scratch_bytes);
+    return BSB_EWORKSPACE;
   }
-  (void)scratch;
-  (void)scratch_bytes;
-  int* status = device_status_word();
-  if (status == nullptr) return BSB_ECUDA;
-  const float scale = 1.0f / sqrtf((float)head_dim);
-  auto go = [&](auto kernel, auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(kernel, dim3(q_heads, batch), dim3(128), 0, (cudaStream_t)stream, (const T*)q, (const T*)k, (const T*)v, q_stride, k_stride,
-                      v_stride, (const T*)cos_table, (const T*)sin_table, table_len, positions, block_table, table_stride, table_width,
-                      (T*)k_pages, (T*)v_pages, num_pages, k_page_stride, v_page_stride, (T*)out, q_heads, kv_heads, page_size, scale, status);
-  };
-  if (dtype == BSB_F16) BSB_CUDA(head_dim == 128 ? go(paged_attention_kernel<__half, 128>, (__half*)nullptr) : go(paged_attention_kernel<__half, 64>, (__half*)nullptr));
-  else BSB_CUDA(head_dim == 128 ? go(paged_attention_kernel<__nv_bfloat16, 128>, (__nv_bfloat16*)nullptr) : go(paged_attention_kernel<__nv_bfloat16, 64>, (__nv_bfloat16*)nullptr));
-  return check_launch("paged_attention_kernel");
+  AttnParams P;
+  P.status = device_status_word();
+  if (P.status == nullptr) return BSB_ECUDA;
+  P.cos_t = cos_table;
+  P.sin_t = sin_table;
+  P.k_pages = k_pages;
+  P.v_pages = v_pages;
+  P.q_stride = q_stride;
+  P.k_stride = k_stride;
+  P.v_stride = v_stride;
+  P.k_page_stride = k_page_stride;
+  P.v_page_stride = v_page_stride;
+  P.table_len = table_len;
+  P.num_pages = num_pages;
+  P.table_stride = table_stride;
+  P.most = (int64_t)table_width * page_size;
+  P.Hq = q_heads;
+  P.Hkv = kv_heads;
+  P.group = q_heads / kv_heads;
+  P.chunks = (P.group + kRows - 1) / kRows;
+  P.rows_kept = P.group < kRows ? P.group : kRows;
+  P.page_size = page_size;
+  P.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
+  P.plan = reinterpret_cast<int4*>(scratch);
+  P.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)sm_count() * 3 * 16);
+  // more requests than a launch keeps prefix sums of: launch after launch, in stream order, on the same scratch
+  for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
+    P.batch = batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch;
+    P.q = (const uint16_t*)q + b0 * q_stride;
+    P.k = (const uint16_t*)k + b0 * k_stride;
+    P.v = (const uint16_t*)v + b0 * v_stride;
+    P.out = (uint16_t*)out + (int64_t)b0 * q_heads * head_dim;
+    P.positions = positions + b0;
+    P.table = block_table + b0 * table_stride;
+    const cudaStream_t s = (cudaStream_t)stream;
+    int rc;
+    if (dtype == BSB_F16) rc = head_dim == 128 ? launch_paged_attention<__half, 128>(P, s) : launch_paged_attention<__half, 64>(P, s);
+    else rc = head_dim == 128 ? launch_paged_attention<__nv_bfloat16, 128>(P, s) : launch_paged_attention<__nv_bfloat16, 64>(P, s);
+    if (rc) return rc;
+  }
+  return BSB_OK;
 }
 
 }  // extern "C"
