@@ -219,7 +219,7 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  *   stays.  uniforms[b] in [0, 1): the token is the first in vocabulary order whose cumulative weight exceeds u times the
  *   total.  temperature <= 0 (or NaN): the first maximum.  NaN logits count as -infinity; a row without a finite logit gives
  *   token 0.  Each of temperature (1), top_k, top_p, min_p may be NULL (off).  logprobs[b] (may be NULL): log of the token's
- *   probability among those kept.  *pos += 1 (pos may be NULL).  Same inputs, same token, bit for bit.  vocab <= 2^20. */
+ *   probability among those kept.  *pos += 1 (pos may be NULL).  Same inputs, same token, bit for bit.  vocab <= 262144. */
 int bsb_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t batch, int32_t* block_table, int64_t table_stride,
                     int32_t table_width, const int32_t* free_pages, const int32_t* free_count, int32_t capacity, int32_t page_size,
                     int64_t max_tokens, int64_t* slots, int64_t* positions, int32_t* offsets, int64_t* last, int32_t* lens_out,

@@ -63,11 +63,12 @@ def test_rope_paged_cache(lib, kw):
 @pytest.mark.parametrize("kw", _BOTH + [dict(d=96), dict(d=256), dict(hq=5), dict(ts=3), dict(tw=0), dict(batch=-1), dict(np=1 << 31)])
 def test_paged_attention(lib, kw):
     assert _attend(lib, **kw) == -1 and lib.bsb_last_error()
-    assert _attend(lib, batch=65536) == -4
+    assert _attend(lib, batch=1 << 30) == -1
+    assert _attend(lib, scb=16) == -3 and _attend(lib, sc=None) == -1 and _attend(lib, sc=ANY + 8) == -1
 
 
 @pytest.mark.parametrize("kw,code", [(dict(vocab=0), -1), (dict(stride=9), -1), (dict(dtype=3), -1), (dict(logits=None), -1), (dict(u=None), -1),
-                                     (dict(tokens=None), -1), (dict(batch=-1), -1), (dict(batch=65536), -4), (dict(vocab=(1 << 20) + 1, stride=1 << 21), -4)])
+                                     (dict(tokens=None), -1), (dict(batch=-1), -1), (dict(batch=(1 << 24) + 1), -4), (dict(vocab=262145, stride=1 << 21), -4)])
 def test_sample_step(lib, kw, code):
     a = dict(logits=ANY, batch=2, vocab=10, stride=10, dtype=0, u=ANY, tokens=ANY)
     a.update(kw)
