@@ -97,6 +97,27 @@ def load():
     return lib
 
 
+_serving = None
+
+
+def serving():
+    """The tensor front end of the serving entry points (csrc/serving_torch.cpp), bound to the loaded library; raises
+    BitStackLibraryError when it is not built."""
+    global _serving
+    if _serving is None:
+        lib = load()
+        import torch  # noqa: F401  (its libraries have to be there first)
+        try:
+            from . import _serving as module
+        except ImportError as e:
+            raise BitStackLibraryError(f"bitstack_b200/_serving.so cannot be loaded ({e}): build it with `python -m bitstack_b200.build`") from e
+        module.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "bsb_page_tables", "bsb_release_pages", "bsb_rope_paged_cache", "bsb_paged_attention_scratch_bytes", "bsb_paged_decode_attention",
+            "bsb_sample_step")})
+        _serving = module
+    return _serving
+
+
 class BitStackDeviceTimeout(BitStackLibraryError):
     """A time-bounded wait inside a kernel gave up; the outputs of that call are NaN."""
 

@@ -3,14 +3,18 @@
     python -m bitstack_b200.build [--force] [--verbose]
 
 The library is a plain C-ABI shared object (see include/bitstack_b200.h); it does
-not link against torch.
+not link against torch.  Beside it, _serving.so is the tensor front end of the serving
+entry points (csrc/serving_torch.cpp): host code only, compiled against torch's headers,
+calling the library through its C ABI.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -18,6 +22,7 @@ LIB = os.path.join(HERE, "libbitstack_b200.so")
 # side build with -DBSB_TUNING: the same library plus timing-experiment modes and a fault-injection mode of the decode
 # kernel (bsb_tuning_set_mode / bsb_tuning_set_trace); the tests of the give-up path load it, the product never does
 TUNING_LIB = os.path.join(HERE, "libbitstack_b200_tuning.so")
+SERVING_LIB = os.path.join(HERE, "_serving.so")
 SOURCES = ["capi.cu", "pack_kernels.cu", "general_kernels.cu", "rebuild_gemm.cu", "gemv_tc5.cu", "gemm_tc5.cu", "signgemm_tc5.cu", "signgemm_mma.cu", "decode_glue.cu", "peer_reduce.cu", "paged.cu", "paged_attention.cu", "sample.cu"]
 HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "rowops.cuh"), os.path.join(CSRC, "numeric.cuh"), os.path.join(os.path.dirname(HERE), "include", "bitstack_b200.h")]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
@@ -66,11 +71,33 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None, lib_path
     return lib_path
 
 
+def build_serving(force: bool = False, verbose: bool = False) -> str:
+    """The tensor front end (host code): g++ against the headers of the torch that this interpreter imports."""
+    src = os.path.join(CSRC, "serving_torch.cpp")
+    if not force and not _stale(SERVING_LIB, [src, HEADERS[-1]]):
+        return SERVING_LIB
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch not found; its headers are required to build the serving front end")
+    torch_dir = spec.submodule_search_locations[0]
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    libs = os.path.join(torch_dir, "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", SERVING_LIB]
+    cmd += ["-I" + p for p in (os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                               sysconfig.get_paths()["include"], os.path.join(cuda, "include"))]
+    cmd += ["-L" + libs, "-Wl,-rpath," + libs, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+    if verbose:
+        sys.stderr.write(" ".join(cmd) + "\n")
+    subprocess.check_call(cmd)
+    return SERVING_LIB
+
+
 def build_tuning(force: bool = False, verbose: bool = False) -> str:
     return build(force=force, verbose=verbose, extra_flags=["-DBSB_TUNING"], lib_path=TUNING_LIB, objdir_name="build_tuning")
 
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    print(build_serving(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
     if "--tuning" in sys.argv:
         print(build_tuning(force="--force" in sys.argv, verbose="--verbose" in sys.argv))

@@ -97,79 +97,8 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor, absmax: torch.Tensor = None) 
 
 
 # ---------------------------------------------------------------------------------- serving over a paged cache
-# These calls are a few microseconds of GPU work at small sizes, so the wrappers are written for the host's time: one
-# comparison per tensor where it is as it should be, and the explanations only where it is not.
-_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _need(t, name: str, dtype, shape, index: int, strided: bool = False) -> None:
-    """Raises ValueError unless `t` is a CUDA tensor on device `index` of this type and shape (None = any extent),
-    contiguous, or with `strided` only in its last dimension."""
-    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == index and t.shape == shape and t.is_contiguous():
-        return
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index:
-        raise ValueError(f"{name} must be a CUDA tensor on cuda:{max(index, 0)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        raise ValueError(f"{name} must have shape {['any' if w is None else w for w in shape]}, got {list(t.shape)}")
-    if not (t.is_contiguous() or (strided and (t.shape[-1] <= 1 or t.stride(-1) == 1))):
-        raise ValueError(f"{name} must be contiguous" + (" in its last dimension" if strided else ""))
-
-
-def _index(t, name: str) -> int:
-    """Device index of a call's first tensor."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    return t.get_device()
-
-
-def _launch(what: str, index: int, *args) -> None:
-    """Calls the library's `what` on the current stream of device `index`, with that device current."""
-    fn = getattr(_lib.load(), what)
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc != 0:
-        _lib.check(rc, what)
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _pages(k_pages, v_pages, dtype, kv_heads, head_dim, index):
-    """(num_pages, page_size, strides of a page) of a cache [num_pages, kv_heads, page_size, head_dim] whose pages are
-    contiguous; the pages themselves may lie apart (one allocation that interleaves K and V, or the layers)."""
-    _need(k_pages, "k_pages", dtype, (None, kv_heads, None, head_dim), index, True)
-    shape = k_pages.shape
-    _need(v_pages, "v_pages", dtype, shape, index, True)
-    n, _, ps, _ = shape
-    if n < 1 or ps < 1:
-        raise ValueError("the page pool is empty")
-    inner = kv_heads * ps * head_dim
-    if k_pages.is_contiguous() and v_pages.is_contiguous():
-        return n, ps, inner, inner
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not t[0].is_contiguous() or (n > 1 and t.stride(0) < inner):
-            raise ValueError(f"{name}: every page [kv_heads, page_size, head_dim] must be contiguous and apart from the next")
-    return n, ps, k_pages.stride(0) if n > 1 else inner, v_pages.stride(0) if n > 1 else inner
-
-
-def _page_lists(lens, block_table, free_pages, free_count):
-    """(device index, requests, width of the table) of the bookkeeping tensors."""
-    index = _index(lens, "lens")
-    batch = lens.shape[0] if lens.dim() == 1 else 0
-    _need(lens, "lens", torch.int32, (batch,), index)
-    width = block_table.shape[-1] if isinstance(block_table, torch.Tensor) and block_table.dim() else 0
-    _need(block_table, "block_table", torch.int32, (batch, width), index, True)
-    _need(free_pages, "free_pages", torch.int32, (None,), index)
-    _need(free_count, "free_count", torch.int32, (1,), index)
-    return index, batch, width
-
+# Argument checks, outputs and scratch are in csrc/serving_torch.cpp: at small sizes these calls are a few microseconds of
+# GPU work, and the same steps take longer than that in Python.
 
 def page_tables(lens, new_tokens, block_table, free_pages, free_count, page_size: int, max_tokens: int = 0, lens_out=None, free_count_out=None):
     """One step of a paged cache's bookkeeping on the device: request b holds lens[b] tokens (int32 [batch]) and gets
@@ -181,92 +110,26 @@ def page_tables(lens, new_tokens, block_table, free_pages, free_count, page_size
     Returns (slots, positions, offsets, last): slot and position of every new token, request after request, int64
     [max_tokens], -1 for tokens of refused requests and behind the end; int32 [batch + 1] first token of every request;
     int64 [batch] position of the request's last new token, -1 when it has none or was refused."""
-    index, batch, width = _page_lists(lens, block_table, free_pages, free_count)
-    _need(new_tokens, "new_tokens", torch.int32, (batch,), index)
-    if lens_out is None:
-        lens_out = lens
-    else:
-        _need(lens_out, "lens_out", torch.int32, (batch,), index)
-    if free_count_out is None:
-        free_count_out = free_count
-    else:
-        _need(free_count_out, "free_count_out", torch.int32, (1,), index)
-    if max_tokens < 0:
-        raise ValueError("max_tokens must not be negative")
-    dev = lens.device
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-    positions = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-    offsets = torch.empty(batch + 1, dtype=torch.int32, device=dev)
-    last = torch.empty(batch, dtype=torch.int64, device=dev)
-    _launch("bsb_page_tables", index, lens.data_ptr(), new_tokens.data_ptr(), batch, block_table.data_ptr(), _row_stride(block_table), width,
-            free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
-            offsets.data_ptr(), last.data_ptr(), lens_out.data_ptr(), free_count_out.data_ptr())
-    return slots, positions, offsets, last
+    return _lib.serving().page_tables(lens, new_tokens, block_table, free_pages, free_count, page_size, max_tokens, lens_out, free_count_out)
 
 
 def release_pages(done, lens, block_table, free_pages, free_count, page_size: int) -> None:
     """Requests with done[b] (bool [batch]) give their pages back to the stack, and their length becomes 0 (in place)."""
-    index, batch, width = _page_lists(lens, block_table, free_pages, free_count)
-    _need(done, "done", torch.bool, (batch,), index)
-    _launch("bsb_release_pages", index, done.data_ptr(), lens.data_ptr(), batch, block_table.data_ptr(), _row_stride(block_table), width,
-            free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size)
-
-
-def _qkv(q, k, v, cos, sin, q_heads, kv_heads, head_dim):
-    dtype = q.dtype if isinstance(q, torch.Tensor) else None
-    if dtype is not torch.float16 and dtype is not torch.bfloat16:
-        raise ValueError(f"q must be fp16 or bf16, got {dtype}")
-    index = _index(q, "q")
-    rows = q.shape[0] if q.dim() else 0
-    _need(q, "q", dtype, (rows, q_heads * head_dim), index, True)
-    _need(k, "k", dtype, (rows, kv_heads * head_dim), index, True)
-    _need(v, "v", dtype, (rows, kv_heads * head_dim), index, True)
-    _need(cos, "cos", dtype, (None, head_dim) if not isinstance(cos, torch.Tensor) or cos.dim() != 2 else (cos.shape[0], head_dim), index)
-    _need(sin, "sin", dtype, cos.shape, index)
-    return index, dtype, rows
+    _lib.serving().release_pages(done, lens, block_table, free_pages, free_count, page_size)
 
 
 def rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages, v_pages, q_heads, kv_heads, head_dim):
     """Rotary embedding of a batch of tokens (a prompt, or several requests' tokens) at `positions` (int64 [tokens]); k and v
     go to `slots` (int64 [tokens]) of k_pages / v_pages [num_pages, kv_heads, page_size, head_dim].  Returns the rotated q
     [tokens, q_heads * head_dim].  Position -1: padding (its q row is 0, nothing is cached); slot -1: not cached."""
-    index, dtype, rows = _qkv(q, k, v, cos, sin, q_heads, kv_heads, head_dim)
-    n, ps, ks, vs = _pages(k_pages, v_pages, dtype, kv_heads, head_dim, index)
-    _need(positions, "positions", torch.int64, (rows,), index)
-    _need(slots, "slots", torch.int64, (rows,), index)
-    out = torch.empty(rows, q_heads * head_dim, dtype=dtype, device=q.device)
-    _launch("bsb_rope_paged_cache", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), _row_stride(q), _row_stride(k), _row_stride(v),
-            cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), n, ks, vs, rows, q_heads, kv_heads, head_dim, ps, _DTYPES[dtype])
-    return out
+    return _lib.serving().rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages, v_pages, q_heads, kv_heads, head_dim)
 
 
 def paged_decode_attention(q, k, v, cos, sin, positions, block_table, k_pages, v_pages, q_heads, kv_heads, head_dim):
     """One new token per request at positions[b] (int64 [batch]; -1: idle row): rotary embedding of q and k, k and v written
     into the request's page (block_table int32 [batch, width]), then grouped-query attention over positions 0 .. positions[b].
     q, k, v: [batch, heads * head_dim], rows may be strided views; fp16 or bf16.  Returns [batch, q_heads * head_dim]."""
-    index, dtype, rows = _qkv(q, k, v, cos, sin, q_heads, kv_heads, head_dim)
-    n, ps, ks, vs = _pages(k_pages, v_pages, dtype, kv_heads, head_dim, index)
-    _need(positions, "positions", torch.int64, (rows,), index)
-    width = block_table.shape[-1] if isinstance(block_table, torch.Tensor) and block_table.dim() else 0
-    _need(block_table, "block_table", torch.int32, (rows, width), index, True)
-    dev = q.device
-    out = torch.empty(rows, q_heads * head_dim, dtype=dtype, device=dev)
-    # scratch of this call alone: from the caching allocator, so that calls on other streams and other captured graphs have theirs
-    need = _attention_scratch.get((index, q_heads, kv_heads, head_dim))
-    if need is None:
-        with torch.cuda.device(index):
-            need = max(_lib.load().bsb_paged_attention_scratch_bytes(rows, q_heads, kv_heads, head_dim), 16)
-        _attention_scratch[(index, q_heads, kv_heads, head_dim)] = need
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-    _launch("bsb_paged_decode_attention", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), _row_stride(q), _row_stride(k), _row_stride(v),
-            cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), block_table.data_ptr(), _row_stride(block_table), width,
-            k_pages.data_ptr(), v_pages.data_ptr(), n, ks, vs, out.data_ptr(), rows, q_heads, kv_heads, head_dim, ps, _DTYPES[dtype],
-            scratch.data_ptr(), need)
-    return out
-
-
-_attention_scratch = {}   # (device, head layout) -> bytes of scratch that one call needs, whatever its batch
+    return _lib.serving().paged_decode_attention(q, k, v, cos, sin, positions, block_table, k_pages, v_pages, q_heads, kv_heads, head_dim)
 
 
 def sample_step(logits, uniforms, tokens, temperature=None, top_k=None, top_p=None, min_p=None, pos=None, logprobs=None):
@@ -275,29 +138,5 @@ def sample_step(logits, uniforms, tokens, temperature=None, top_k=None, top_p=No
     pos[0] += 1 (skipped when pos is None).  logits: [batch, vocab] fp16, bf16 or fp32 with unit inner stride.
     temperature 0: the first maximum, as `greedy_step`.  `logprobs` (fp32 [batch], optional) receives the log of the
     token's probability among those kept."""
-    dtype = logits.dtype if isinstance(logits, torch.Tensor) else None
-    if dtype not in _DTYPES:
-        raise ValueError(f"logits must be fp16, bf16 or fp32, got {dtype}")
-    index = _index(logits, "logits")
-    _need(logits, "logits", dtype, (None, None), index, True)
-    batch, vocab = logits.shape
-    row = (batch,)
-    _need(uniforms, "uniforms", torch.float32, row, index)
-    _need(tokens, "tokens", torch.int64, row, index)
-    if temperature is not None:
-        _need(temperature, "temperature", torch.float32, row, index)
-    if top_k is not None:
-        _need(top_k, "top_k", torch.int32, row, index)
-    if top_p is not None:
-        _need(top_p, "top_p", torch.float32, row, index)
-    if min_p is not None:
-        _need(min_p, "min_p", torch.float32, row, index)
-    if logprobs is not None:
-        _need(logprobs, "logprobs", torch.float32, row, index)
-    if pos is not None:
-        _need(pos, "pos", torch.int64, (1,), index)
-    _launch("bsb_sample_step", index, logits.data_ptr(), batch, vocab, _row_stride(logits), _DTYPES[dtype], uniforms.data_ptr(),
-            None if temperature is None else temperature.data_ptr(), None if top_k is None else top_k.data_ptr(),
-            None if top_p is None else top_p.data_ptr(), None if min_p is None else min_p.data_ptr(), tokens.data_ptr(),
-            None if pos is None else pos.data_ptr(), None if logprobs is None else logprobs.data_ptr())
+    _lib.serving().sample_step(logits, uniforms, tokens, temperature, top_k, top_p, min_p, pos, logprobs)
     return tokens

@@ -11,8 +11,9 @@ ANY = 1 << 20   # a non-null, aligned address: refused calls never follow it
 
 @pytest.fixture(scope="module")
 def lib():
-    from bitstack_b200.build import build
+    from bitstack_b200.build import build, build_serving
     build()
+    build_serving()
     return _lib.load()
 
 
@@ -83,7 +84,7 @@ def test_nothing_to_do_is_fine(lib):
     assert lib.bsb_paged_attention_scratch_bytes(4, 5, 2, 128) == -1
 
 
-def test_wrappers_refuse_host_tensors():
+def test_wrappers_refuse_host_tensors(lib):
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
         glue.page_tables(i, i, torch.zeros(2, 3, dtype=torch.int32), i, torch.zeros(1, dtype=torch.int32), 16)
