@@ -9,9 +9,12 @@
 //  * A CTA is four warps, and a warp is on its own: it streams its 16 positions of every tile through a ring of its own in
 //    shared memory (16-byte cp.async, rows looked up page by page, so a page may end anywhere) and needs no barrier with the
 //    others until the pair ends.  Rows behind the last position are filled with zeros, whatever the page holds there.
-//  * All query heads of a group (up to 16, the M of mma.sync m16n8k16) share the K and V that were read; scores and output are
-//    accumulated in fp32, the weights are rounded to the cache's type for the second product (half a step of relative error
-//    each, as q is rounded after its rotation), and one pass keeps the running maximum and sum.
+//  * All query heads of a group share the K and V that were read.  The products are taken transposed, scores^T = K Q^T and
+//    output^T = V^T P^T, so that positions and dimensions fill the 16 rows of mma.sync m16n8k16 and the heads its 8 columns: a
+//    group of up to 8 heads wastes nothing (half the MMAs, exponentials and accumulators of the untransposed form), one of up
+//    to 16 takes two column blocks.  Scores and output are accumulated in fp32, the weights are rounded to the cache's type for
+//    the second product (half a step of relative error each, as q is rounded after its rotation), and one pass keeps the
+//    running maximum and sum.
 //  * The new position's K and V come from the projection's output: turned, stored to the page and to the ring by the warp
 //    that meets the position, so nothing is read back.
 #include <climits>
@@ -25,13 +28,19 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16 * kWarps;       // positions of a tile
-constexpr int kRows = 16;                // query heads of one pass (the M of the MMA)
+constexpr int kRows = 16;                // most query heads of one pass
 constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix sums stay in shared memory
 constexpr int64_t kWholePositions = 512; // requests that cannot be longer than this get one CTA per (request, kv head): no join
-
+#ifndef BSB_ATTN_STAGES
+#define BSB_ATTN_STAGES 2
+#endif
+#ifndef BSB_ATTN_CTAS
+#define BSB_ATTN_CTAS 3
+#endif
 template <int D> struct Shape;
-template <> struct Shape<128> { static constexpr int stages = 3, ctas = 2; };
-template <> struct Shape<64> { static constexpr int stages = 4, ctas = 3; };
+template <> struct Shape<128> { static constexpr int stages = BSB_ATTN_STAGES, ctas = BSB_ATTN_CTAS; };
+template <> struct Shape<64> { static constexpr int stages = 2 * BSB_ATTN_STAGES, ctas = BSB_ATTN_CTAS; };
+constexpr int kMaxCtas = 4;              // per multiprocessor, for the scratch
 
 struct AttnParams {
   const void *q, *k, *v, *cos_t, *sin_t;
@@ -39,11 +48,13 @@ struct AttnParams {
   int64_t q_stride, k_stride, v_stride, k_page_stride, v_page_stride, table_len, num_pages, table_stride;
   const int64_t* positions;
   const int32_t* table;
-  int64_t most;                          // positions that a table row can hold
+  int64_t most;                          // positions that a table row can hold, at most 2^31 - 64
   int batch, Hq, Hkv, group, chunks, rows_kept, page_size;
+  uint32_t page_mul, page_shift;         // p / page_size = (p * page_mul) >> page_shift for p < 2^31
+  int whole;                             // one CTA per (request, kv head)
   float scale_log2;
   float* part;                           // [CTA][2]: 16 maxima, 16 sums, rows_kept x D outputs (every part 16-byte aligned)
-  int4* plan;                            // [CTA]: first output row, heads, last CTA of the shared pair that begins in this CTA; heads == 0: none
+  int4* plan;                            // [CTA]: first output row, heads, last CTA of the shared pair that begins in this CTA; no heads: none
   int* status;
 };
 
@@ -68,6 +79,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // an 8 x 8 block of 16-bit values across the warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -80,19 +96,38 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // tokens a request holds after this step; -1: its position is behind its table row or the cos / sin tables
-__device__ __forceinline__ int64_t length_of(const AttnParams& P, int b) {
+__device__ __forceinline__ int length_of(const AttnParams& P, int b) {
   const int64_t pos = P.positions[b];
   if (pos < 0) return 0;
-  return pos < P.most && pos < P.table_len ? pos + 1 : -1;
+  return pos < P.most && pos < P.table_len ? (int)pos + 1 : -1;
 }
-__device__ __forceinline__ int64_t tiles_of(int64_t n) { return n <= 0 ? 1 : (n + kTile - 1) / kTile; }   // idle rows too have an output
+__device__ __forceinline__ int tiles_of(int n) { return n <= 0 ? 1 : (n + kTile - 1) / kTile; }   // idle rows too have an output
+
+// rotary embedding of eight pairs (i, i + D/2): x*cos + rotate_half(x)*sin with rotate_half(x) = [-x1, x0]
+template <typename T, int D>
+__device__ __forceinline__ void turn8(const T* src, const T* cos_t, const T* sin_t, float (&x0)[8], float (&x1)[8]) {
+  float c0[8], c1[8], s0[8], s1[8];
+  load8(src, x0);
+  load8(src + D / 2, x1);
+  load8(cos_t, c0);
+  load8(cos_t + D / 2, c1);
+  load8(sin_t, s0);
+  load8(sin_t + D / 2, s1);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float a = x0[e], b = x1[e];
+    x0[e] = a * c0[e] - b * s0[e];
+    x1[e] = b * c1[e] + a * s1[e];
+  }
+}
 
 // dynamic shared memory: [warp][stage][K 16 rows, V 16 rows], q [16 rows], maxima and sums [2][warp][16], prefix sums [batch + 1]
 template <int D> constexpr int ring_bytes() { return kWarps * Shape<D>::stages * 2 * 16 * D * 2; }
 template <int D> constexpr int fixed_bytes() { return ring_bytes<D>() + kRows * D * 2 + 2 * kWarps * kRows * 4; }
 
-template <typename T, int D, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kernel(const __grid_constant__ AttnParams P) {
+// NB: column blocks of 8 heads.  ALIGNED: pages are a multiple of 16 rows, so the 16 positions of a warp lie in one page.
+template <typename T, int D, int NB, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_attention_kernel(const __grid_constant__ AttnParams P) {
   constexpr int kStages = Shape<D>::stages;
   constexpr int kChunks = D / 8;                 // 16-byte pieces of a row
   constexpr int kStep = 32 / kChunks;            // rows that one warp-wide copy covers
@@ -109,9 +144,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kern
 
   // ---- this CTA's share of the tiles ------------------------------------------------------------------------------
   int64_t first, end, share = 0;
-  int b, pair;
-  int64_t t0 = 0;
-  if (WHOLE) {
+  int b, pair, t0 = 0;
+  if (P.whole) {
     b = blockIdx.x / pairs;
     pair = blockIdx.x - b * pairs;
     first = 0;
@@ -149,120 +183,103 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kern
       else h = mid - 1;
     }
     b = l;
-    const int64_t in = first - s_before[b] * pairs, tiles = s_before[b + 1] - s_before[b];
+    const int64_t in = first - s_before[b] * pairs;
+    const int tiles = (int)(s_before[b + 1] - s_before[b]);
     pair = (int)(in / tiles);
-    t0 = in - pair * tiles;
+    t0 = (int)(in - (int64_t)pair * tiles);
   }
 
   uint8_t* ring = smem + warp * (kStages * 2 * kHalf);
   const uint32_t ring_at = smem_u32(ring);
   const int gid = lane >> 2, t4 = lane & 3;
   const float nan = __int_as_float(0x7FC00000);
+  // this lane's piece of a warp-wide copy: rows copy_row, copy_row + kStep, ..; the swizzle of a row r is r & 7
+  const int copy_row = lane / kChunks, copy_c = lane % kChunks;
 
   for (int64_t at = first; at < end;) {
-    const int64_t len = length_of(P, b);
-    const int64_t n = max(len, (int64_t)0);
-    const int64_t tiles = tiles_of(len);
-    const int nt = (int)min(tiles - t0, end - at);                 // tiles of this pair that are this CTA's
+    const int len = length_of(P, b), n = max(len, 0), tiles = tiles_of(len);
+    const int nt = (int)min((int64_t)(tiles - t0), end - at);      // tiles of this pair that are this CTA's
     const int hk = pair / P.chunks, head0 = hk * P.group + (pair - hk * P.chunks) * kRows;
     const int heads = min(kRows, (hk + 1) * P.group - head0);
     const int32_t* pages = P.table + (int64_t)b * P.table_stride;
+    const T* cos_t = (const T*)P.cos_t + (int64_t)(n - 1) * D;
+    const T* sin_t = (const T*)P.sin_t + (int64_t)(n - 1) * D;
     bool bad = len < 0;
 
-    // ---- q: turned, rounded to the type, rows behind the group zero ------------------------------------------------
-    for (int it = tid; it < kRows * (D / 16); it += kThreads) {
-      const int r = it / (D / 16), c = it - r * (D / 16);
-      float x0[8], x1[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
-      if (r < heads && n > 0) {
-        const T* src = (const T*)P.q + b * P.q_stride + (int64_t)(head0 + r) * D + c * 8;
-        float c0[8], c1[8], s0[8], s1[8];
-        load8(src, x0);
-        load8(src + D / 2, x1);
-        load8((const T*)P.cos_t + (n - 1) * D + c * 8, c0);
-        load8((const T*)P.cos_t + (n - 1) * D + c * 8 + D / 2, c1);
-        load8((const T*)P.sin_t + (n - 1) * D + c * 8, s0);
-        load8((const T*)P.sin_t + (n - 1) * D + c * 8 + D / 2, s1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a = x0[e], d = x1[e];
-          x0[e] = a * c0[e] - d * s0[e];
-          x1[e] = d * c1[e] + a * s1[e];
-        }
-      }
-      *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((c ^ (r & 7)) << 4)) = pack8<T>(x0);
-      *reinterpret_cast<uint4*>(s_q + r * D * 2 + (((c + D / 16) ^ (r & 7)) << 4)) = pack8<T>(x1);
-    }
-    __syncthreads();
-    uint32_t qf[D / 16][4];
-    {
-      const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) ldsm4(smem_u32(s_q) + r * D * 2 + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4), qf[ks]);
-    }
-
-    // ---- the ring: lane r (and r + 16) knows where row r of the tile to come lies ------------------------------------
-    const int64_t base0 = t0 * kTile + warp * 16;
+    // ---- the ring ------------------------------------------------------------------------------------------------------
+    const int base0 = t0 * kTile + warp * 16;
+    auto page_of = [&](int p) { return (int)(((uint64_t)(uint32_t)p * P.page_mul) >> P.page_shift); };
     int page_next = 0;
-    auto look_up = [&](int i) {                   // page of this lane's row in tile i of the share; loaded one tile ahead of its use
-      const int64_t p = base0 + (int64_t)i * kTile + (lane & 15);
-      page_next = i < nt && p < n ? pages[p / P.page_size] : 0;
+    // ALIGNED: the page of the 16 positions; else lane r (and r + 16) that of row r.  Loaded one tile ahead of its use.
+    auto look_up = [&](int i) {
+      const int p = base0 + i * kTile + (ALIGNED ? 0 : lane & 15);
+      page_next = i < nt && p < n ? pages[page_of(p)] : 0;
     };
     auto issue = [&](int i) {
-      if (i < nt) {
-        const int64_t p = base0 + (int64_t)i * kTile + (lane & 15);
+      const int base = base0 + i * kTile;
+      if (i < nt && base < n) {
         const int page = page_next;
-        const bool valid = p < n;
-        const bool found = valid && page >= 0 && page < P.num_pages;
-        if (valid && !found) bad = true;
-        const int in_page = (int)(p % P.page_size);
-        const bool fresh = p == n - 1;
-        const int code = fresh ? -2 : found ? page : -1;   // -2: written below, -1: zeros
         look_up(i + 1);
         const uint32_t dst = ring_at + (i % kStages) * (2 * kHalf);
+        const int fresh = n - 1 - base;           // row of the new position, if it is one of these 16
+        int fresh_page, fresh_row;                // where it is stored
+        if (ALIGNED) {
+          const bool found = page >= 0 && page < P.num_pages;
+          bad |= !found;
+          const int in_page = base - page_of(base) * P.page_size;
+          const int64_t off = ((int64_t)hk * P.page_size + in_page + copy_row) * D + copy_c * 8;
+          const T* ks = (const T*)P.k_pages + (found ? page * P.k_page_stride + off : 0);
+          const T* vs = (const T*)P.v_pages + (found ? page * P.v_page_stride + off : 0);
+          const int step = found ? kStep * D : 0;
 #pragma unroll
-        for (int j = 0; j < 16; j += kStep) {
-          const int r = j + lane / kChunks, c = lane % kChunks;
-          const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
-          const bool keep = pg >= 0;
-          const int64_t off = ((int64_t)hk * P.page_size + rw) * D + c * 8;
-          const uint32_t d = dst + r * D * 2 + ((c ^ (r & 7)) << 4);
-          const T* ks = (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0);
-          const T* vs = (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0);
-          if (pg != -2) {
-            cp_async16(d, ks, keep);
-            cp_async16(d + kHalf, vs, keep);
-          }
-        }
-        // the new position: in the last tile only
-        const uint32_t who = __ballot_sync(0xFFFFFFFFu, fresh && lane < 16);
-        if (who != 0) {
-          const int r = __ffs(who) - 1;
-          const int pg = __shfl_sync(0xFFFFFFFFu, found ? page : -1, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
-          const bool write = pg >= 0 && pair == hk * P.chunks;
-          const int64_t off = ((int64_t)hk * P.page_size + rw) * D;
-          T* kd = (T*)P.k_pages + (write ? pg * P.k_page_stride + off : 0);
-          T* vd = (T*)P.v_pages + (write ? pg * P.v_page_stride + off : 0);
-          uint8_t* row = ring + (i % kStages) * (2 * kHalf) + r * D * 2;
-          if (lane < D / 16) {
-            const T* src = (const T*)P.k + b * P.k_stride + (int64_t)hk * D + lane * 8;
-            float x0[8], x1[8], c0[8], c1[8], s0[8], s1[8];
-            load8(src, x0);
-            load8(src + D / 2, x1);
-            load8((const T*)P.cos_t + (n - 1) * D + lane * 8, c0);
-            load8((const T*)P.cos_t + (n - 1) * D + lane * 8 + D / 2, c1);
-            load8((const T*)P.sin_t + (n - 1) * D + lane * 8, s0);
-            load8((const T*)P.sin_t + (n - 1) * D + lane * 8 + D / 2, s1);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = x0[e], d = x1[e];
-              x0[e] = a * c0[e] - d * s0[e];
-              x1[e] = d * c1[e] + a * s1[e];
+          for (int j = 0; j < 16; j += kStep) {
+            const int r = j + copy_row;
+            const uint32_t d = dst + r * D * 2 + ((copy_c ^ (r & 7)) << 4);
+            if (r != fresh) {                     // rows behind the last position: zeros
+              cp_async16(d, ks, found && r < fresh);
+              cp_async16(d + kHalf, vs, found && r < fresh);
             }
+            if (r + kStep < fresh) {              // (the source moves on only where the next row is one to be read)
+              ks += step;
+              vs += step;
+            }
+          }
+          fresh_page = found ? page : -1;
+          fresh_row = in_page + fresh;
+        } else {
+          const int p = base + (lane & 15);
+          const bool valid = p < n, found = valid && page >= 0 && page < P.num_pages;
+          bad |= valid && !found;
+          const int in_page = p - page_of(p) * P.page_size;
+          const int code = found ? page : -1;
+#pragma unroll
+          for (int j = 0; j < 16; j += kStep) {
+            const int r = j + copy_row;
+            const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
+            const bool keep = pg >= 0 && r < fresh;
+            const int64_t off = ((int64_t)hk * P.page_size + rw) * D + copy_c * 8;
+            const uint32_t d = dst + r * D * 2 + ((copy_c ^ (r & 7)) << 4);
+            if (r != fresh) {
+              cp_async16(d, (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0), keep);
+              cp_async16(d + kHalf, (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0), keep);
+            }
+          }
+          fresh_page = __shfl_sync(0xFFFFFFFFu, code, fresh & 15);
+          fresh_row = __shfl_sync(0xFFFFFFFFu, in_page, fresh & 15);
+        }
+        if (fresh < 16) {                         // the new position: turned, stored to the page and to the ring
+          const bool write = fresh_page >= 0 && pair == hk * P.chunks;
+          const int64_t off = ((int64_t)hk * P.page_size + fresh_row) * D;
+          T* kd = (T*)P.k_pages + (write ? fresh_page * P.k_page_stride + off : 0);
+          T* vd = (T*)P.v_pages + (write ? fresh_page * P.v_page_stride + off : 0);
+          uint8_t* row = ring + (i % kStages) * (2 * kHalf) + fresh * D * 2;
+          const int sw = fresh & 7;
+          if (lane < D / 16) {
+            float x0[8], x1[8];
+            turn8<T, D>((const T*)P.k + b * P.k_stride + (int64_t)hk * D + lane * 8, cos_t + lane * 8, sin_t + lane * 8, x0, x1);
             const uint4 lo = pack8<T>(x0), hi = pack8<T>(x1);
-            *reinterpret_cast<uint4*>(row + ((lane ^ (r & 7)) << 4)) = lo;
-            *reinterpret_cast<uint4*>(row + (((lane + D / 16) ^ (r & 7)) << 4)) = hi;
+            *reinterpret_cast<uint4*>(row + ((lane ^ sw) << 4)) = lo;
+            *reinterpret_cast<uint4*>(row + (((lane + D / 16) ^ sw) << 4)) = hi;
             if (write) {
               *reinterpret_cast<uint4*>(kd + lane * 8) = lo;
               *reinterpret_cast<uint4*>(kd + lane * 8 + D / 2) = hi;
@@ -270,91 +287,130 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kern
           } else if (lane >= 16 && lane < 16 + D / 8) {
             const int c = lane - 16;
             const uint4 x = *reinterpret_cast<const uint4*>((const T*)P.v + b * P.v_stride + (int64_t)hk * D + c * 8);
-            *reinterpret_cast<uint4*>(row + kHalf + ((c ^ (r & 7)) << 4)) = x;
+            *reinterpret_cast<uint4*>(row + kHalf + ((c ^ sw) << 4)) = x;
             if (write) *reinterpret_cast<uint4*>(vd + c * 8) = x;
           }
         }
       }
       cp_async_commit();
     };
-
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[D / 8][4];
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-
     look_up(0);
 #pragma unroll
     for (int i = 0; i < kStages; ++i) issue(i);
+
+    // ---- q: turned, rounded to the type, rows behind the group zero ------------------------------------------------
+    for (int it = tid; it < NB * 8 * (D / 16); it += kThreads) {
+      const int r = it / (D / 16), c = it - r * (D / 16);
+      float x0[8], x1[8];
+      if (r < heads && n > 0) {
+        turn8<T, D>((const T*)P.q + b * P.q_stride + (int64_t)(head0 + r) * D + c * 8, cos_t + c * 8, sin_t + c * 8, x0, x1);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
+      }
+      *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((c ^ (r & 7)) << 4)) = pack8<T>(x0);
+      *reinterpret_cast<uint4*>(s_q + r * D * 2 + (((c + D / 16) ^ (r & 7)) << 4)) = pack8<T>(x1);
+    }
+    __syncthreads();
+    uint32_t qf[NB][D / 32][4];                   // columns = heads: two k steps per load
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+      const int r = h * 8 + (lane & 7);
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) ldsm4(smem_u32(s_q) + r * D * 2 + (((4 * ks + (lane >> 3)) ^ (r & 7)) << 4), qf[h][ks]);
+    }
+
+    // heads 8h + 2 t4 and + 1 of this lane: running maximum (of the raw scores) and sum; output^T, rows = dimensions
+    float m[NB][2], l[NB][2], o[NB][D / 16][4];
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+      m[h][0] = m[h][1] = -INFINITY;
+      l[h][0] = l[h][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[h][j][e] = 0.f;
+    }
     for (int i = 0; i < nt; ++i) {
       cp_async_wait<kStages - 1>();
       __syncwarp();
-      const int64_t base = base0 + (int64_t)i * kTile;
-      if (base < n) {
+      const int left = n - (base0 + i * kTile);   // positions of these 16 that exist, if positive
+      if (left > 0) {
         const uint32_t kt = ring_at + (i % kStages) * (2 * kHalf), vt = kt + kHalf;
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        {
-          const int r = (lane & 7) + (lane >> 4) * 8;
+        float s[NB][4];                           // (position gid, heads), (position gid + 8, heads)
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            uint32_t kf[4];
-            ldsm4(kt + r * D * 2 + (((2 * ks + ((lane >> 3) & 1)) ^ (r & 7)) << 4), kf);
-            mma16816<T>(s[0], qf[ks], kf[0], kf[1]);
-            mma16816<T>(s[1], qf[ks], kf[2], kf[3]);
-          }
-        }
-        const int left = (int)min(n - base, (int64_t)16);   // positions of these 16 that exist
-        float x0 = -INFINITY, x1 = -INFINITY;
+        for (int h = 0; h < NB; ++h)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bool in = h * 8 + t4 * 2 + e < left;
-            s[h][e] = in ? s[h][e] * P.scale_log2 : -INFINITY;
-            s[h][e + 2] = in ? s[h][e + 2] * P.scale_log2 : -INFINITY;
-            x0 = fmaxf(x0, s[h][e]);
-            x1 = fmaxf(x1, s[h][e + 2]);
-          }
-#pragma unroll
-        for (int w = 1; w < 4; w <<= 1) {
-          x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, w));
-          x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, w));
-        }
-        x0 = fmaxf(x0, m0);                       // finite: at least one position exists
-        x1 = fmaxf(x1, m1);
-        if (__any_sync(0xFFFFFFFFu, x0 > m0 || x1 > m1)) {
-          const float f0 = fast_exp2(m0 - x0), f1 = fast_exp2(m1 - x1);
-          l0 *= f0;
-          l1 *= f1;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            o[j][0] *= f0;
-            o[j][1] *= f0;
-            o[j][2] *= f1;
-            o[j][3] *= f1;
-          }
-          m0 = x0;
-          m1 = x1;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            s[h][e] = fast_exp2(s[h][e] - m0);
-            s[h][e + 2] = fast_exp2(s[h][e + 2] - m1);
-            l0 += s[h][e];
-            l1 += s[h][e + 2];
-          }
-        const uint32_t pf[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+          for (int e = 0; e < 4; ++e) s[h][e] = 0.f;
         {
           const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-          for (int j = 0; j < D / 8; j += 2) {
+          for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t kf[4];
+            ldsm4(kt + r * D * 2 + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4), kf);
+#pragma unroll
+            for (int h = 0; h < NB; ++h) mma16816<T>(s[h], kf, qf[h][ks / 2][(ks & 1) * 2], qf[h][ks / 2][(ks & 1) * 2 + 1]);
+          }
+        }
+        if (left < 16) {
+#pragma unroll
+          for (int h = 0; h < NB; ++h) {
+            if (gid >= left) s[h][0] = s[h][1] = -INFINITY;
+            if (gid + 8 >= left) s[h][2] = s[h][3] = -INFINITY;
+          }
+        }
+        float x[NB][2];
+        bool moved = false;
+#pragma unroll
+        for (int h = 0; h < NB; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[h][e] = fmaxf(s[h][e], s[h][e + 2]);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) x[h][e] = fmaxf(x[h][e], __shfl_xor_sync(0xFFFFFFFFu, x[h][e], w));
+            moved |= x[h][e] > m[h][e];
+          }
+        if (__any_sync(0xFFFFFFFFu, moved)) {
+#pragma unroll
+          for (int h = 0; h < NB; ++h) {
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float top = fmaxf(x[h][e], m[h][e]);
+              f[e] = fast_exp2((m[h][e] - top) * P.scale_log2);
+              m[h][e] = top;
+              l[h][e] *= f[e];
+            }
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+              o[h][j][0] *= f[0];
+              o[h][j][1] *= f[1];
+              o[h][j][2] *= f[0];
+              o[h][j][3] *= f[1];
+            }
+          }
+        }
+        uint32_t pf[NB][2];                       // weights^T: rows = positions, columns = heads
+#pragma unroll
+        for (int h = 0; h < NB; ++h) {
+          const float c0 = -m[h][0] * P.scale_log2, c1 = -m[h][1] * P.scale_log2;
+          s[h][0] = fast_exp2(fmaf(s[h][0], P.scale_log2, c0));
+          s[h][1] = fast_exp2(fmaf(s[h][1], P.scale_log2, c1));
+          s[h][2] = fast_exp2(fmaf(s[h][2], P.scale_log2, c0));
+          s[h][3] = fast_exp2(fmaf(s[h][3], P.scale_log2, c1));
+          l[h][0] += s[h][0] + s[h][2];
+          l[h][1] += s[h][1] + s[h][3];
+          pf[h][0] = transpose8(pack2<T>(s[h][0], s[h][1]));
+          pf[h][1] = transpose8(pack2<T>(s[h][2], s[h][3]));
+        }
+        {
+          const int r = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
             uint32_t vf[4];
-            ldsm4_t(vt + r * D * 2 + (((j + (lane >> 4)) ^ (r & 7)) << 4), vf);
-            mma16816<T>(o[j], pf, vf[0], vf[1]);
-            mma16816<T>(o[j + 1], pf, vf[2], vf[3]);
+            ldsm4_t(vt + r * D * 2 + (((2 * j + ((lane >> 3) & 1)) ^ (r & 7)) << 4), vf);
+#pragma unroll
+            for (int h = 0; h < NB; ++h) mma16816<T>(o[h][j], vf, pf[h][0], pf[h][1]);
           }
         }
       }
@@ -367,49 +423,51 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kern
     bad = __syncthreads_or(bad);                  // (also: q may be overwritten from here on)
 
     // ---- the four warps' results, joined ------------------------------------------------------------------------------
+    float* mine = reinterpret_cast<float*>(ring);   // [heads][D] fp32, no more than the ring: dimension d of head r at d ^ 8 (r & 7)
 #pragma unroll
-    for (int w = 1; w < 4; w <<= 1) {
-      l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, w);
-      l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, w);
-    }
-    if (t4 == 0) {
-      s_m[warp * kRows + gid] = m0;
-      s_m[warp * kRows + gid + 8] = m1;
-      s_l[warp * kRows + gid] = l0;
-      s_l[warp * kRows + gid + 8] = l1;
-    }
-    float* mine = reinterpret_cast<float*>(ring);   // [16][D] fp32: no more than a ring of two stages
+    for (int h = 0; h < NB; ++h)
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      const int col = (j * 8 + t4 * 2) ^ (gid * 8 & (D - 1));   // rows shifted against one another: no bank conflicts
-      if (gid < heads) *reinterpret_cast<float2*>(mine + gid * D + col) = make_float2(o[j][0], o[j][1]);
-      if (gid + 8 < heads) *reinterpret_cast<float2*>(mine + (gid + 8) * D + col) = make_float2(o[j][2], o[j][3]);
-    }
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[h][e] += __shfl_xor_sync(0xFFFFFFFFu, l[h][e], w);
+        const int r = h * 8 + t4 * 2 + e;
+        if (gid == 0) {
+          s_m[warp * kRows + r] = m[h][e] * P.scale_log2;
+          s_l[warp * kRows + r] = l[h][e];
+        }
+        if (r < heads) {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            mine[r * D + ((j * 16 + gid) ^ ((r & 7) * 8))] = o[h][j][e];
+            mine[r * D + ((j * 16 + gid + 8) ^ ((r & 7) * 8))] = o[h][j][e + 2];
+          }
+        }
+      }
     __syncthreads();
     const bool begins = t0 == 0, ends = t0 + nt == tiles;
     const int slot_floats = 2 * kRows + P.rows_kept * D;
-    float* part = WHOLE ? nullptr : P.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * slot_floats;
+    float* part = P.whole ? nullptr : P.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * slot_floats;
     const int64_t out_row = (int64_t)b * P.Hq + head0;
     for (int it = tid; it < heads * (D / 4); it += kThreads) {
       const int r = it / (D / 4), c = (it - r * (D / 4)) * 4;
-      float m = s_m[r];
+      float top = s_m[r];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w * kRows + r]);
-      float l = 0.f;
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * kRows + r]);
+      float sum = 0.f;
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float mw = s_m[w * kRows + r], f = mw == -INFINITY ? 0.f : fast_exp2(mw - m);
-        const float4 x = *reinterpret_cast<const float4*>(smem + w * (kStages * 2 * kHalf) + (r * D + (c ^ ((r & 7) * 8 & (D - 1)))) * 4);
-        l += s_l[w * kRows + r] * f;
+        const float mw = s_m[w * kRows + r], f = mw == -INFINITY ? 0.f : fast_exp2(mw - top);
+        const float4 x = *reinterpret_cast<const float4*>(smem + w * (kStages * 2 * kHalf) + (r * D + (c ^ ((r & 7) * 8))) * 4);
+        sum += s_l[w * kRows + r] * f;
         a.x += x.x * f;
         a.y += x.y * f;
         a.z += x.z * f;
         a.w += x.w * f;
       }
-      if (bad) l = nan;
+      if (bad) sum = nan;
       if (begins && ends) {
-        const float inv = n > 0 || bad ? 1.f / l : 0.f;            // idle: zeros
+        const float inv = n > 0 || bad ? 1.f / sum : 0.f;          // idle: zeros
         uint2 packed;
         packed.x = pack2<T>(a.x * inv, a.y * inv);
         packed.y = pack2<T>(a.z * inv, a.w * inv);
@@ -417,12 +475,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas) paged_attention_kern
       } else {
         *reinterpret_cast<float4*>(part + 2 * kRows + r * D + c) = a;
         if (c == 0) {
-          part[r] = m;
-          part[kRows + r] = l;
+          part[r] = top;
+          part[kRows + r] = sum;
         }
       }
     }
-    if (!WHOLE && begins && !ends && tid == 0) {   // this CTA's last pair: the CTAs behind hold the rest of it
+    if (begins && !ends && tid == 0) {            // this CTA's last pair: the CTAs behind hold the rest of it
       const int64_t pair_end = at + tiles;
       P.plan[blockIdx.x] = make_int4((int)out_row, heads, (int)((pair_end - 1) / share), 0);
     }
@@ -462,28 +520,32 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int NB, bool ALIGNED>
 int launch_paged_attention(AttnParams P, cudaStream_t s) {
+  constexpr int kCtas = NB == 1 ? Shape<D>::ctas : 2;
   const int pairs = P.Hkv * P.chunks;
-  const bool whole = P.most <= kWholePositions;
-  const int grid = whole ? P.batch * pairs : sm_count() * Shape<D>::ctas;
-  const size_t smem = fixed_bytes<D>() + (whole ? 0 : (size_t)(P.batch + 1) * 8);
+  P.whole = P.most <= kWholePositions;
+  const int grid = P.whole ? P.batch * pairs : sm_count() * kCtas;
+  const size_t smem = fixed_bytes<D>() + (P.whole ? 0 : (size_t)(P.batch + 1) * 8);
   static bool attr_set[64] = {false};
   int dev = 0;
   BSB_CUDA(cudaGetDevice(&dev));
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed_bytes<D>() + (kMaxBatch + 1) * 8));
-    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed_bytes<D>()));
+    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, NB, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  fixed_bytes<D>() + (kMaxBatch + 1) * 8));
     attr_set[dev] = true;
   }
-  if (whole) {
-    BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, true>, dim3(grid), dim3(kThreads), smem, s, P));
-    return check_launch("paged_attention_kernel");
-  }
-  BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, false>, dim3(grid), dim3(kThreads), smem, s, P));
+  BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, NB, ALIGNED>, dim3(grid), dim3(kThreads), smem, s, P));
   if (int rc = check_launch("paged_attention_kernel")) return rc;
+  if (P.whole) return BSB_OK;
   BSB_CUDA(launch_pdl(paged_attention_join_kernel<T, D>, dim3(grid), dim3(256), 0, s, P));
   return check_launch("paged_attention_join_kernel");
+}
+template <typename T, int D>
+int launch_paged_attention(const AttnParams& P, cudaStream_t s) {
+  const bool aligned = P.page_size % 16 == 0;
+  if (P.group <= 8) return aligned ? launch_paged_attention<T, D, 1, true>(P, s) : launch_paged_attention<T, D, 1, false>(P, s);
+  return aligned ? launch_paged_attention<T, D, 2, true>(P, s) : launch_paged_attention<T, D, 2, false>(P, s);
 }
 
 }  // namespace
@@ -496,7 +558,7 @@ extern "C" {
 int64_t bsb_paged_attention_scratch_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (batch < 0 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || q_heads % kv_heads != 0) return -1;
   const int rows = q_heads / kv_heads < kRows ? q_heads / kv_heads : kRows;
-  return (int64_t)sm_count() * 3 * (16 + 2 * (2 * kRows + (int64_t)rows * head_dim) * 4);
+  return (int64_t)sm_count() * kMaxCtas * (16 + 2 * (2 * kRows + (int64_t)rows * head_dim) * 4);
 }
 
 int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -541,6 +603,10 @@ int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int6
   P.num_pages = num_pages;
   P.table_stride = table_stride;
   P.most = (int64_t)table_width * page_size;
+  if (P.most > INT_MAX - 63) P.most = INT_MAX - 63;
+  P.page_shift = 31;                     // mul = ceil(2^shift / page_size) < 2^32 with 2^(shift - 31) >= page_size: exact below 2^31
+  while ((1ll << (P.page_shift - 31)) < page_size) ++P.page_shift;
+  P.page_mul = (uint32_t)(((1ull << P.page_shift) + page_size - 1) / page_size);
   P.Hq = q_heads;
   P.Hkv = kv_heads;
   P.group = q_heads / kv_heads;
@@ -549,7 +615,7 @@ int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int6
   P.page_size = page_size;
   P.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   P.plan = reinterpret_cast<int4*>(scratch);
-  P.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)sm_count() * 3 * 16);
+  P.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)sm_count() * kMaxCtas * 16);
   // more requests than a launch keeps prefix sums of: launch after launch, in stream order, on the same scratch
   for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
     P.batch = batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch;
