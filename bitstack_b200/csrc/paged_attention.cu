@@ -30,16 +30,11 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16 * kWarps;       // positions of a tile
 constexpr int kRows = 16;                // most query heads of one pass
 constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix sums stay in shared memory
+constexpr float kSlack = 6.f;            // see the running maximum
 constexpr int64_t kWholePositions = 512; // requests that cannot be longer than this get one CTA per (request, kv head): no join
-#ifndef BSB_ATTN_STAGES
-#define BSB_ATTN_STAGES 2
-#endif
-#ifndef BSB_ATTN_CTAS
-#define BSB_ATTN_CTAS 3
-#endif
-template <int D> struct Shape;
-template <> struct Shape<128> { static constexpr int stages = BSB_ATTN_STAGES, ctas = BSB_ATTN_CTAS; };
-template <> struct Shape<64> { static constexpr int stages = 2 * BSB_ATTN_STAGES, ctas = BSB_ATTN_CTAS; };
+template <int D> struct Shape;           // stages of a warp's ring, CTAs of a multiprocessor
+template <> struct Shape<128> { static constexpr int stages = 2, ctas = 3; };
+template <> struct Shape<64> { static constexpr int stages = 3, ctas = 4; };
 constexpr int kMaxCtas = 4;              // per multiprocessor, for the scratch
 
 struct AttnParams {
@@ -61,6 +56,9 @@ struct AttnParams {
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool keep) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(keep ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -132,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
   constexpr int kChunks = D / 8;                 // 16-byte pieces of a row
   constexpr int kStep = 32 / kChunks;            // rows that one warp-wide copy covers
   constexpr int kHalf = 16 * D * 2;              // bytes of the K (or V) rows of a stage
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* s_q = smem + ring_bytes<D>();
   float* s_m = reinterpret_cast<float*>(s_q + kRows * D * 2);
   float* s_l = s_m + kWarps * kRows;
@@ -195,6 +193,11 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
   const float nan = __int_as_float(0x7FC00000);
   // this lane's piece of a warp-wide copy: rows copy_row, copy_row + kStep, ..; the swizzle of a row r is r & 7
   const int copy_row = lane / kChunks, copy_c = lane % kChunks;
+  const uint32_t ring_copy = ring_at + copy_row * D * 2 + ((copy_c ^ copy_row) << 4);
+  // where this lane's rows of K (row = position) and V (transposed) fragments begin; pieces 2j on are 32 j bytes on, swizzled alike
+  const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
+  const uint32_t k_frag = ring_at + k_row * D * 2 + (((lane >> 4) ^ (k_row & 7)) << 4);
+  const uint32_t v_frag = ring_at + kHalf + v_row * D * 2 + ((((lane >> 3) & 1) ^ (v_row & 7)) << 4);
 
   for (int64_t at = first; at < end;) {
     const int len = length_of(P, b), n = max(len, 0), tiles = tiles_of(len);
@@ -220,53 +223,38 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
       if (i < nt && base < n) {
         const int page = page_next;
         look_up(i + 1);
-        const uint32_t dst = ring_at + (i % kStages) * (2 * kHalf);
+        const uint32_t dst = ring_copy + (i % kStages) * (2 * kHalf);
         const int fresh = n - 1 - base;           // row of the new position, if it is one of these 16
-        int fresh_page, fresh_row;                // where it is stored
-        if (ALIGNED) {
-          const bool found = page >= 0 && page < P.num_pages;
-          bad |= !found;
-          const int in_page = base - page_of(base) * P.page_size;
-          const int64_t off = ((int64_t)hk * P.page_size + in_page + copy_row) * D + copy_c * 8;
-          const T* ks = (const T*)P.k_pages + (found ? page * P.k_page_stride + off : 0);
-          const T* vs = (const T*)P.v_pages + (found ? page * P.v_page_stride + off : 0);
-          const int step = found ? kStep * D : 0;
+        if (ALIGNED && fresh >= 16 && page >= 0 && page < P.num_pages) {   // 16 rows of one page: nothing to decide
+          const int64_t off = ((int64_t)hk * P.page_size + (base - page_of(base) * P.page_size) + copy_row) * D + copy_c * 8;
+          const T* ks = (const T*)P.k_pages + page * P.k_page_stride + off;
+          const T* vs = (const T*)P.v_pages + page * P.v_page_stride + off;
 #pragma unroll
-          for (int j = 0; j < 16; j += kStep) {
-            const int r = j + copy_row;
-            const uint32_t d = dst + r * D * 2 + ((copy_c ^ (r & 7)) << 4);
-            if (r != fresh) {                     // rows behind the last position: zeros
-              cp_async16(d, ks, found && r < fresh);
-              cp_async16(d + kHalf, vs, found && r < fresh);
-            }
-            if (r + kStep < fresh) {              // (the source moves on only where the next row is one to be read)
-              ks += step;
-              vs += step;
-            }
+          for (int j = 0; j < 16; j += kStep) {   // (the swizzle of row j + copy_row is that of copy_row, turned by j)
+            cp_async16((dst + j * D * 2) ^ ((j & 7) << 4), ks + j * D);
+            cp_async16((dst + kHalf + j * D * 2) ^ ((j & 7) << 4), vs + j * D);
           }
-          fresh_page = found ? page : -1;
-          fresh_row = in_page + fresh;
-        } else {
-          const int p = base + (lane & 15);
-          const bool valid = p < n, found = valid && page >= 0 && page < P.num_pages;
-          bad |= valid && !found;
-          const int in_page = p - page_of(p) * P.page_size;
-          const int code = found ? page : -1;
-#pragma unroll
-          for (int j = 0; j < 16; j += kStep) {
-            const int r = j + copy_row;
-            const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
-            const bool keep = pg >= 0 && r < fresh;
-            const int64_t off = ((int64_t)hk * P.page_size + rw) * D + copy_c * 8;
-            const uint32_t d = dst + r * D * 2 + ((copy_c ^ (r & 7)) << 4);
-            if (r != fresh) {
-              cp_async16(d, (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0), keep);
-              cp_async16(d + kHalf, (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0), keep);
-            }
-          }
-          fresh_page = __shfl_sync(0xFFFFFFFFu, code, fresh & 15);
-          fresh_row = __shfl_sync(0xFFFFFFFFu, in_page, fresh & 15);
+          cp_async_commit();
+          return;
         }
+        const int p = base + (lane & 15);
+        const bool valid = p < n, found = valid && page >= 0 && page < P.num_pages;
+        bad |= valid && !found;
+        const int in_page = p - page_of(p) * P.page_size;
+        const int code = found ? page : -1;
+#pragma unroll
+        for (int j = 0; j < 16; j += kStep) {
+          const int r = j + copy_row;
+          const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
+          const bool keep = pg >= 0 && r < fresh;
+          const int64_t off = ((int64_t)hk * P.page_size + rw) * D + copy_c * 8;
+          const uint32_t d = (dst + j * D * 2) ^ ((j & 7) << 4);
+          if (r != fresh) {                       // rows behind the last position: zeros
+            cp_async16(d, (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0), keep);
+            cp_async16(d + kHalf, (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0), keep);
+          }
+        }
+        const int fresh_page = __shfl_sync(0xFFFFFFFFu, code, fresh & 15), fresh_row = __shfl_sync(0xFFFFFFFFu, in_page, fresh & 15);
         if (fresh < 16) {                         // the new position: turned, stored to the page and to the ring
           const bool write = fresh_page >= 0 && pair == hk * P.chunks;
           const int64_t off = ((int64_t)hk * P.page_size + fresh_row) * D;
@@ -321,10 +309,11 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     }
 
     // heads 8h + 2 t4 and + 1 of this lane: running maximum (of the raw scores) and sum; output^T, rows = dimensions
-    float m[NB][2], l[NB][2], o[NB][D / 16][4];
+    float m[NB][2], limit[NB][2], l[NB][2], o[NB][D / 16][4];
+    const float slack = kSlack / P.scale_log2;
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
-      m[h][0] = m[h][1] = -INFINITY;
+      m[h][0] = m[h][1] = limit[h][0] = limit[h][1] = -INFINITY;
       l[h][0] = l[h][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
@@ -336,21 +325,18 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
       __syncwarp();
       const int left = n - (base0 + i * kTile);   // positions of these 16 that exist, if positive
       if (left > 0) {
-        const uint32_t kt = ring_at + (i % kStages) * (2 * kHalf), vt = kt + kHalf;
+        const uint32_t stage = (i % kStages) * (2 * kHalf);
         float s[NB][4];                           // (position gid, heads), (position gid + 8, heads)
 #pragma unroll
         for (int h = 0; h < NB; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[h][e] = 0.f;
-        {
-          const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            uint32_t kf[4];
-            ldsm4(kt + r * D * 2 + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4), kf);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t kf[4];
+          ldsm4((k_frag + stage) ^ (ks << 5), kf);
 #pragma unroll
-            for (int h = 0; h < NB; ++h) mma16816<T>(s[h], kf, qf[h][ks / 2][(ks & 1) * 2], qf[h][ks / 2][(ks & 1) * 2 + 1]);
-          }
+          for (int h = 0; h < NB; ++h) mma16816<T>(s[h], kf, qf[h][ks / 2][(ks & 1) * 2], qf[h][ks / 2][(ks & 1) * 2 + 1]);
         }
         if (left < 16) {
 #pragma unroll
@@ -359,26 +345,26 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
             if (gid + 8 >= left) s[h][2] = s[h][3] = -INFINITY;
           }
         }
-        float x[NB][2];
+        // The reference that the exponents are taken against moves only when a score has passed it by more than 2^kSlack:
+        // weights up to that are as exact in every type here, and most tiles need no reduction over the positions.
         bool moved = false;
 #pragma unroll
         for (int h = 0; h < NB; ++h)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            x[h][e] = fmaxf(s[h][e], s[h][e + 2]);
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) x[h][e] = fmaxf(x[h][e], __shfl_xor_sync(0xFFFFFFFFu, x[h][e], w));
-            moved |= x[h][e] > m[h][e];
-          }
+          for (int e = 0; e < 2; ++e) moved |= fmaxf(s[h][e], s[h][e + 2]) > limit[h][e];
         if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
           for (int h = 0; h < NB; ++h) {
             float f[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float top = fmaxf(x[h][e], m[h][e]);
+              float top = fmaxf(s[h][e], s[h][e + 2]);
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
+              top = fmaxf(top, m[h][e]);
               f[e] = fast_exp2((m[h][e] - top) * P.scale_log2);
               m[h][e] = top;
+              limit[h][e] = top + slack;
               l[h][e] *= f[e];
             }
 #pragma unroll
@@ -403,15 +389,12 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
           pf[h][0] = transpose8(pack2<T>(s[h][0], s[h][1]));
           pf[h][1] = transpose8(pack2<T>(s[h][2], s[h][3]));
         }
-        {
-          const int r = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            uint32_t vf[4];
-            ldsm4_t(vt + r * D * 2 + (((2 * j + ((lane >> 3) & 1)) ^ (r & 7)) << 4), vf);
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t vf[4];
+          ldsm4_t((v_frag + stage) ^ (j << 5), vf);
 #pragma unroll
-            for (int h = 0; h < NB; ++h) mma16816<T>(o[h][j], vf, pf[h][0], pf[h][1]);
-          }
+          for (int h = 0; h < NB; ++h) mma16816<T>(o[h][j], vf, pf[h][0], pf[h][1]);
         }
       }
       __syncwarp();                               // every lane has read the stage before it is filled again
