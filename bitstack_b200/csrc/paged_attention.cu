@@ -30,6 +30,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16 * kWarps;       // positions of a tile
 constexpr int kRows = 16;                // most query heads of one pass
 constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix sums stay in shared memory
+constexpr int kPairCost = 3;             // what a pair costs a CTA beside its tiles, in tiles
 constexpr float kSlack = 6.f;            // see the running maximum
 constexpr int64_t kWholePositions = 512; // requests that cannot be longer than this get one CTA per (request, kv head): no join
 template <int D> struct Shape;           // stages of a warp's ring, CTAs of a multiprocessor
@@ -49,7 +50,8 @@ struct AttnParams {
   int whole;                             // one CTA per (request, kv head)
   float scale_log2;
   float* part;                           // [CTA][2]: 16 maxima, 16 sums, rows_kept x D outputs (every part 16-byte aligned)
-  int4* plan;                            // [CTA]: first output row, heads, last CTA of the shared pair that begins in this CTA; no heads: none
+  int4* plan;                            // [CTA][2]: pairs shared with other CTAs, the one that this CTA continues and the one that begins
+                                         // in it: first output row, heads (0: there is none), first and last CTA
   int* status;
 };
 
@@ -93,6 +95,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
+// a / b, in 32 bits where they do (a 64-bit division is a long chain of instructions)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 // tokens a request holds after this step; -1: its position is behind its table row or the cos / sin tables
 __device__ __forceinline__ int length_of(const AttnParams& P, int b) {
   const int64_t pos = P.positions[b];
@@ -138,11 +144,14 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
   __shared__ int64_t s_sum[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int pairs = P.Hkv * P.chunks;            // (kv head, chunk of its query heads)
-  pdl_enter();
+  pdl_wait();   // (the join is let in at the end: its waiting CTAs cost this kernel 10 % when they come early)
 
   // ---- this CTA's share of the tiles ------------------------------------------------------------------------------
+  // The sequence is counted in units: a pair is kPairCost units in front of its tiles.  Short requests then do not pile up in one
+  // CTA's share, where each of them would cost a round of latencies for a tile or two.
   int64_t first, end, share = 0;
-  int b, pair, t0 = 0;
+  int b, pair, u0 = 0;
+  const int cost = P.whole ? 0 : kPairCost;
   if (P.whole) {
     b = blockIdx.x / pairs;
     pair = blockIdx.x - b * pairs;
@@ -152,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     const int each = (P.batch + kThreads - 1) / kThreads;
     const int lo = min(tid * each, P.batch), hi = min(lo + each, P.batch);
     int64_t mine = 0;
-    for (int i = lo; i < hi; ++i) mine += tiles_of(length_of(P, i));
+    for (int i = lo; i < hi; ++i) mine += cost + tiles_of(length_of(P, i));
     int64_t upto = mine;
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
@@ -164,17 +173,18 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     int64_t run = upto - mine;
     for (int i = lo; i < hi; ++i) {
       s_before[i] = run;
-      run += tiles_of(length_of(P, i));
+      run += cost + tiles_of(length_of(P, i));
     }
     if (tid == kThreads - 1) s_before[P.batch] = upto;
     __syncthreads();
     const int64_t total = s_before[P.batch] * pairs;
-    share = (total + gridDim.x - 1) / gridDim.x;
+    share = divide(total + gridDim.x - 1, gridDim.x);
     first = min(blockIdx.x * share, total);
     end = min(first + share, total);
-    if (tid == 0) P.plan[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid < 2) P.plan[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
+    __syncthreads();                             // (thread 0 may fill in either of them)
     if (first == end) return;
-    int l = 0, h = P.batch - 1;                  // the request of tile `first`
+    int l = 0, h = P.batch - 1;                  // the request of unit `first`
     while (l < h) {
       const int mid = (l + h + 1) >> 1;
       if (s_before[mid] * pairs <= first) l = mid;
@@ -182,9 +192,10 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     }
     b = l;
     const int64_t in = first - s_before[b] * pairs;
-    const int tiles = (int)(s_before[b + 1] - s_before[b]);
-    pair = (int)(in / tiles);
-    t0 = (int)(in - (int64_t)pair * tiles);
+    const int units = (int)(s_before[b + 1] - s_before[b]);
+    pair = (int)divide(in, units);
+    u0 = (int)(in - (int64_t)pair * units);
+    if (u0 + (end - first) <= cost) return;      // nothing but the cost of a pair that begins further on
   }
 
   uint8_t* ring = smem + warp * (kStages * 2 * kHalf);
@@ -199,94 +210,109 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
   const uint32_t k_frag = ring_at + k_row * D * 2 + (((lane >> 4) ^ (k_row & 7)) << 4);
   const uint32_t v_frag = ring_at + kHalf + v_row * D * 2 + ((((lane >> 3) & 1) ^ (v_row & 7)) << 4);
 
-  for (int64_t at = first; at < end;) {
-    const int len = length_of(P, b), n = max(len, 0), tiles = tiles_of(len);
-    const int nt = (int)min((int64_t)(tiles - t0), end - at);      // tiles of this pair that are this CTA's
-    const int hk = pair / P.chunks, head0 = hk * P.group + (pair - hk * P.chunks) * kRows;
-    const int heads = min(kRows, (hk + 1) * P.group - head0);
-    const int32_t* pages = P.table + (int64_t)b * P.table_stride;
-    const T* cos_t = (const T*)P.cos_t + (int64_t)(n - 1) * D;
-    const T* sin_t = (const T*)P.sin_t + (int64_t)(n - 1) * D;
-    bool bad = len < 0;
+  // ---- the stretch of one pair that is worked on: tiles t0 .. t0 + nt - 1 of request b, units u0 .. u0 + used - 1 of the pair, from
+  // unit `at` of the sequence
+  int64_t at = first;
+  int n, tiles, t0, nt, used, hk, head0, heads, base0;
+  const int32_t* pages;
+  const T *cos_t, *sin_t;
+  bool bad;
+  auto enter = [&]() {
+    const int len = length_of(P, b);
+    n = max(len, 0);
+    bad = len < 0;
+    tiles = tiles_of(len);
+    used = (int)min((int64_t)(tiles + cost - u0), end - at);
+    t0 = max(u0 - cost, 0);
+    nt = u0 + used - cost - t0;
+    hk = pair / P.chunks;
+    head0 = hk * P.group + (pair - hk * P.chunks) * kRows;
+    heads = min(kRows, (hk + 1) * P.group - head0);
+    base0 = t0 * kTile + warp * 16;
+    pages = P.table + (int64_t)b * P.table_stride;
+    cos_t = (const T*)P.cos_t + (int64_t)(n - 1) * D;
+    sin_t = (const T*)P.sin_t + (int64_t)(n - 1) * D;
+  };
+  enter();
 
-    // ---- the ring ------------------------------------------------------------------------------------------------------
-    const int base0 = t0 * kTile + warp * 16;
-    auto page_of = [&](int p) { return (int)(((uint64_t)(uint32_t)p * P.page_mul) >> P.page_shift); };
-    int page_next = 0;
-    // ALIGNED: the page of the 16 positions; else lane r (and r + 16) that of row r.  Loaded one tile ahead of its use.
-    auto look_up = [&](int i) {
-      const int p = base0 + i * kTile + (ALIGNED ? 0 : lane & 15);
-      page_next = i < nt && p < n ? pages[page_of(p)] : 0;
-    };
-    auto issue = [&](int i) {
-      const int base = base0 + i * kTile;
-      if (i < nt && base < n) {
-        const int page = page_next;
-        look_up(i + 1);
-        const uint32_t dst = ring_copy + (i % kStages) * (2 * kHalf);
-        const int fresh = n - 1 - base;           // row of the new position, if it is one of these 16
-        if (ALIGNED && fresh >= 16 && page >= 0 && page < P.num_pages) {   // 16 rows of one page: nothing to decide
-          const int64_t off = ((int64_t)hk * P.page_size + (base - page_of(base) * P.page_size) + copy_row) * D + copy_c * 8;
-          const T* ks = (const T*)P.k_pages + page * P.k_page_stride + off;
-          const T* vs = (const T*)P.v_pages + page * P.v_page_stride + off;
+  // ---- the ring ------------------------------------------------------------------------------------------------------
+  auto page_of = [&](int p) { return (int)(((uint64_t)(uint32_t)p * P.page_mul) >> P.page_shift); };
+  int page_next = 0;
+  // Tile i of a stretch goes to stage (i + 1) % stages.  All but the last stage's worth of a stretch is asked for while the one
+  // before it is being joined, which uses stage 0.
+  auto stage_of = [&](int i) { return (uint32_t)((i + 1) % kStages) * (2 * kHalf); };
+  // ALIGNED: the page of the 16 positions; else lane r (and r + 16) that of row r.  Loaded one tile ahead of its use.
+  auto look_up = [&](int i) {
+    const int p = base0 + i * kTile + (ALIGNED ? 0 : lane & 15);
+    page_next = i < nt && p < n ? pages[page_of(p)] : 0;
+  };
+  auto issue = [&](int i) {
+    const int base = base0 + i * kTile;
+    if (i < nt && base < n) {
+      const int page = page_next;
+      look_up(i + 1);
+      const uint32_t dst = ring_copy + stage_of(i);
+      const int fresh = n - 1 - base;           // row of the new position, if it is one of these 16
+      if (ALIGNED && fresh >= 16 && page >= 0 && page < P.num_pages) {   // 16 rows of one page: nothing to decide
+        const int64_t off = ((int64_t)hk * P.page_size + (base - page_of(base) * P.page_size) + copy_row) * D + copy_c * 8;
+        const T* ks = (const T*)P.k_pages + page * P.k_page_stride + off;
+        const T* vs = (const T*)P.v_pages + page * P.v_page_stride + off;
 #pragma unroll
-          for (int j = 0; j < 16; j += kStep) {   // (the swizzle of row j + copy_row is that of copy_row, turned by j)
-            cp_async16((dst + j * D * 2) ^ ((j & 7) << 4), ks + j * D);
-            cp_async16((dst + kHalf + j * D * 2) ^ ((j & 7) << 4), vs + j * D);
-          }
-          cp_async_commit();
-          return;
+        for (int j = 0; j < 16; j += kStep) {   // (the swizzle of row j + copy_row is that of copy_row, turned by j)
+          cp_async16((dst + j * D * 2) ^ ((j & 7) << 4), ks + j * D);
+          cp_async16((dst + kHalf + j * D * 2) ^ ((j & 7) << 4), vs + j * D);
         }
-        const int p = base + (lane & 15);
-        const bool valid = p < n, found = valid && page >= 0 && page < P.num_pages;
-        bad |= valid && !found;
-        const int in_page = p - page_of(p) * P.page_size;
-        const int code = found ? page : -1;
+        cp_async_commit();
+        return;
+      }
+      const int p = base + (lane & 15);
+      const bool valid = p < n, found = valid && page >= 0 && page < P.num_pages;
+      bad |= valid && !found;
+      const int in_page = p - page_of(p) * P.page_size;
+      const int code = found ? page : -1;
 #pragma unroll
-        for (int j = 0; j < 16; j += kStep) {
-          const int r = j + copy_row;
-          const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
-          const bool keep = pg >= 0 && r < fresh;
-          const int64_t off = ((int64_t)hk * P.page_size + rw) * D + copy_c * 8;
-          const uint32_t d = (dst + j * D * 2) ^ ((j & 7) << 4);
-          if (r != fresh) {                       // rows behind the last position: zeros
-            cp_async16(d, (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0), keep);
-            cp_async16(d + kHalf, (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0), keep);
-          }
-        }
-        const int fresh_page = __shfl_sync(0xFFFFFFFFu, code, fresh & 15), fresh_row = __shfl_sync(0xFFFFFFFFu, in_page, fresh & 15);
-        if (fresh < 16) {                         // the new position: turned, stored to the page and to the ring
-          const bool write = fresh_page >= 0 && pair == hk * P.chunks;
-          const int64_t off = ((int64_t)hk * P.page_size + fresh_row) * D;
-          T* kd = (T*)P.k_pages + (write ? fresh_page * P.k_page_stride + off : 0);
-          T* vd = (T*)P.v_pages + (write ? fresh_page * P.v_page_stride + off : 0);
-          uint8_t* row = ring + (i % kStages) * (2 * kHalf) + fresh * D * 2;
-          const int sw = fresh & 7;
-          if (lane < D / 16) {
-            float x0[8], x1[8];
-            turn8<T, D>((const T*)P.k + b * P.k_stride + (int64_t)hk * D + lane * 8, cos_t + lane * 8, sin_t + lane * 8, x0, x1);
-            const uint4 lo = pack8<T>(x0), hi = pack8<T>(x1);
-            *reinterpret_cast<uint4*>(row + ((lane ^ sw) << 4)) = lo;
-            *reinterpret_cast<uint4*>(row + (((lane + D / 16) ^ sw) << 4)) = hi;
-            if (write) {
-              *reinterpret_cast<uint4*>(kd + lane * 8) = lo;
-              *reinterpret_cast<uint4*>(kd + lane * 8 + D / 2) = hi;
-            }
-          } else if (lane >= 16 && lane < 16 + D / 8) {
-            const int c = lane - 16;
-            const uint4 x = *reinterpret_cast<const uint4*>((const T*)P.v + b * P.v_stride + (int64_t)hk * D + c * 8);
-            *reinterpret_cast<uint4*>(row + kHalf + ((c ^ sw) << 4)) = x;
-            if (write) *reinterpret_cast<uint4*>(vd + c * 8) = x;
-          }
+      for (int j = 0; j < 16; j += kStep) {
+        const int r = j + copy_row;
+        const int pg = __shfl_sync(0xFFFFFFFFu, code, r), rw = __shfl_sync(0xFFFFFFFFu, in_page, r);
+        const bool keep = pg >= 0 && r < fresh;
+        const int64_t off = ((int64_t)hk * P.page_size + rw) * D + copy_c * 8;
+        const uint32_t d = (dst + j * D * 2) ^ ((j & 7) << 4);
+        if (r != fresh) {                       // rows behind the last position: zeros
+          cp_async16(d, (const T*)P.k_pages + (keep ? pg * P.k_page_stride + off : 0), keep);
+          cp_async16(d + kHalf, (const T*)P.v_pages + (keep ? pg * P.v_page_stride + off : 0), keep);
         }
       }
-      cp_async_commit();
-    };
-    look_up(0);
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) issue(i);
+      const int fresh_page = __shfl_sync(0xFFFFFFFFu, code, fresh & 15), fresh_row = __shfl_sync(0xFFFFFFFFu, in_page, fresh & 15);
+      if (fresh < 16) {                         // the new position: turned, stored to the page and to the ring
+        const bool write = fresh_page >= 0 && pair == hk * P.chunks;
+        const int64_t off = ((int64_t)hk * P.page_size + fresh_row) * D;
+        T* kd = (T*)P.k_pages + (write ? fresh_page * P.k_page_stride + off : 0);
+        T* vd = (T*)P.v_pages + (write ? fresh_page * P.v_page_stride + off : 0);
+        uint8_t* row = ring + stage_of(i) + fresh * D * 2;
+        const int sw = fresh & 7;
+        if (lane < D / 16) {
+          float x0[8], x1[8];
+          turn8<T, D>((const T*)P.k + b * P.k_stride + (int64_t)hk * D + lane * 8, cos_t + lane * 8, sin_t + lane * 8, x0, x1);
+          const uint4 lo = pack8<T>(x0), hi = pack8<T>(x1);
+          *reinterpret_cast<uint4*>(row + ((lane ^ sw) << 4)) = lo;
+          *reinterpret_cast<uint4*>(row + (((lane + D / 16) ^ sw) << 4)) = hi;
+          if (write) {
+            *reinterpret_cast<uint4*>(kd + lane * 8) = lo;
+            *reinterpret_cast<uint4*>(kd + lane * 8 + D / 2) = hi;
+          }
+        } else if (lane >= 16 && lane < 16 + D / 8) {
+          const int c = lane - 16;
+          const uint4 x = *reinterpret_cast<const uint4*>((const T*)P.v + b * P.v_stride + (int64_t)hk * D + c * 8);
+          *reinterpret_cast<uint4*>(row + kHalf + ((c ^ sw) << 4)) = x;
+          if (write) *reinterpret_cast<uint4*>(vd + c * 8) = x;
+        }
+      }
+    }
+    cp_async_commit();
+  };
 
-    // ---- q: turned, rounded to the type, rows behind the group zero ------------------------------------------------
+  // ---- q: turned, rounded to the type, rows behind the group zero ------------------------------------------------
+  auto stage_q = [&]() {
     for (int it = tid; it < NB * 8 * (D / 16); it += kThreads) {
       const int r = it / (D / 16), c = it - r * (D / 16);
       float x0[8], x1[8];
@@ -299,7 +325,19 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
       *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((c ^ (r & 7)) << 4)) = pack8<T>(x0);
       *reinterpret_cast<uint4*>(s_q + r * D * 2 + (((c + D / 16) ^ (r & 7)) << 4)) = pack8<T>(x1);
     }
-    __syncthreads();
+  };
+
+  auto begin = [&]() {
+    look_up(0);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+  };
+  begin();
+  stage_q();
+  __syncthreads();
+  issue(kStages - 1);
+
+  while (true) {
     uint32_t qf[NB][D / 32][4];                   // columns = heads: two k steps per load
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
@@ -325,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
       __syncwarp();
       const int left = n - (base0 + i * kTile);   // positions of these 16 that exist, if positive
       if (left > 0) {
-        const uint32_t stage = (i % kStages) * (2 * kHalf);
+        const uint32_t stage = stage_of(i);
         float s[NB][4];                           // (position gid, heads), (position gid + 8, heads)
 #pragma unroll
         for (int h = 0; h < NB; ++h)
@@ -402,10 +440,21 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     }
     cp_async_wait<0>();
     __syncwarp();
-    if (bad) atomicCAS(P.status, 0, 61);
-    bad = __syncthreads_or(bad);                  // (also: q may be overwritten from here on)
-
-    // ---- the four warps' results, joined ------------------------------------------------------------------------------
+    // ---- on to the next stretch, while this one's results are joined -----------------------------------------------------
+    const int done_n = n, done_heads = heads;
+    const bool begins = t0 == 0, ends = t0 + nt == tiles, last = at + used + cost >= end;
+    const int64_t pair_begin = at - u0 + cost, pair_end = pair_begin + tiles, out_row = (int64_t)b * P.Hq + head0;
+    const bool failed = bad;
+    if (!last) {
+      at += used;
+      u0 = 0;
+      if (++pair == pairs) {
+        pair = 0;
+        ++b;
+      }
+      enter();
+      begin();
+    }
     float* mine = reinterpret_cast<float*>(ring);   // [heads][D] fp32, no more than the ring: dimension d of head r at d ^ 8 (r & 7)
 #pragma unroll
     for (int h = 0; h < NB; ++h)
@@ -418,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
           s_m[warp * kRows + r] = m[h][e] * P.scale_log2;
           s_l[warp * kRows + r] = l[h][e];
         }
-        if (r < heads) {
+        if (r < done_heads) {
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
             mine[r * D + ((j * 16 + gid) ^ ((r & 7) * 8))] = o[h][j][e];
@@ -426,12 +475,11 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
           }
         }
       }
-    __syncthreads();
-    const bool begins = t0 == 0, ends = t0 + nt == tiles;
+    if (failed) atomicCAS(P.status, 0, 61);
+    const bool any_failed = __syncthreads_or(failed);
     const int slot_floats = 2 * kRows + P.rows_kept * D;
     float* part = P.whole ? nullptr : P.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * slot_floats;
-    const int64_t out_row = (int64_t)b * P.Hq + head0;
-    for (int it = tid; it < heads * (D / 4); it += kThreads) {
+    for (int it = tid; it < done_heads * (D / 4); it += kThreads) {
       const int r = it / (D / 4), c = (it - r * (D / 4)) * 4;
       float top = s_m[r];
 #pragma unroll
@@ -448,9 +496,9 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
         a.z += x.z * f;
         a.w += x.w * f;
       }
-      if (bad) sum = nan;
+      if (any_failed) sum = nan;
       if (begins && ends) {
-        const float inv = n > 0 || bad ? 1.f / sum : 0.f;          // idle: zeros
+        const float inv = done_n > 0 || any_failed ? 1.f / sum : 0.f;          // idle: zeros
         uint2 packed;
         packed.x = pack2<T>(a.x * inv, a.y * inv);
         packed.y = pack2<T>(a.z * inv, a.w * inv);
@@ -463,43 +511,68 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
         }
       }
     }
-    if (begins && !ends && tid == 0) {            // this CTA's last pair: the CTAs behind hold the rest of it
-      const int64_t pair_end = at + tiles;
-      P.plan[blockIdx.x] = make_int4((int)out_row, heads, (int)((pair_end - 1) / share), 0);
+    if (!(begins && ends) && tid == 0)
+      P.plan[2 * blockIdx.x + (begins ? 1 : 0)] = make_int4((int)out_row, done_heads, (int)divide(pair_begin, share), (int)divide(pair_end - 1, share));
+    if (last) {
+      pdl_trigger();
+      return;
     }
-    __syncthreads();                              // the ring is free again
-    at += nt;
-    t0 = 0;
-    if (++pair == pairs) {
-      pair = 0;
-      ++b;
-    }
+    stage_q();
+    __syncthreads();                              // stage 0 is free again, and q is there
+    issue(kStages - 1);
   }
 }
 
-// shared pairs: CTA c joins the pair that began in c's share and ends in that of plan[c].z
+// Pairs that several CTAs share: each of them joins a slice of the outputs.  A float4 of an output is added up by as many
+// lanes as there are parts (up to 32), so that all loads of a slice are in flight at once.
+constexpr int kJoinThreads = 128;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_attention_join_kernel(const __grid_constant__ AttnParams P) {
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ AttnParams P) {
   pdl_enter();
-  const int c0 = blockIdx.x;
-  const int4 plan = P.plan[c0];
   const int slot = 2 * kRows + P.rows_kept * D;
-  for (int it = threadIdx.x; it < plan.y * (D / 2); it += blockDim.x) {
-    const int r = it / (D / 2), c = (it - r * (D / 2)) * 2;
-    float m = P.part[((int64_t)c0 * 2 + 1) * slot + r];
-    for (int i = c0 + 1; i <= plan.z; ++i) m = fmaxf(m, P.part[(int64_t)i * 2 * slot + r]);
-    float l = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 4
-    for (int i = c0; i <= plan.z; ++i) {
-      const float* part = P.part + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * slot;
-      const float f = fast_exp2(part[r] - m);
-      const float2 o = *reinterpret_cast<const float2*>(part + 2 * kRows + r * D + c);
-      l += part[kRows + r] * f;
-      x += o.x * f;
-      y += o.y * f;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int4 plan = P.plan[2 * blockIdx.x + which];
+    if (plan.y == 0) continue;
+    const int c0 = plan.z, count = plan.w - plan.z + 1, units = plan.y * (D / 4);
+    const int lo = (int)((int64_t)units * ((int)blockIdx.x - c0) / count), hi = (int)((int64_t)units * ((int)blockIdx.x - c0 + 1) / count);
+    int lanes = 2;                                // of a unit
+    while (lanes < 32 && lanes < count) lanes *= 2;
+    const int sub = threadIdx.x % lanes;
+    for (int u0 = lo; u0 < hi; u0 += kJoinThreads / lanes) {   // the same trips for the whole CTA
+      const int u = min(u0 + (int)threadIdx.x / lanes, hi - 1), r = u / (D / 4), c = (u - r * (D / 4)) * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = sub; i < count; i += lanes) {
+        const float* part = P.part + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * slot;
+        const float mi = part[r], li = part[kRows + r];
+        const float4 o = *reinterpret_cast<const float4*>(part + 2 * kRows + r * D + c);
+        const float top = fmaxf(m, mi);
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top), g = mi == -INFINITY ? 0.f : fast_exp2(mi - top);
+        m = top;
+        l = l * f + li * g;
+        a = make_float4(a.x * f + o.x * g, a.y * f + o.y * g, a.z * f + o.z * g, a.w * f + o.w * g);
+      }
+      float top = m;
+      for (int w = 1; w < lanes; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+      l *= f;
+      a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+      for (int w = 1; w < lanes; w <<= 1) {
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, w);
+        a.x += __shfl_xor_sync(0xFFFFFFFFu, a.x, w);
+        a.y += __shfl_xor_sync(0xFFFFFFFFu, a.y, w);
+        a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, w);
+        a.w += __shfl_xor_sync(0xFFFFFFFFu, a.w, w);
+      }
+      if (sub == 0 && u0 + (int)threadIdx.x / lanes < hi) {
+        const float inv = 1.f / l;
+        uint2 packed;
+        packed.x = pack2<T>(a.x * inv, a.y * inv);
+        packed.y = pack2<T>(a.z * inv, a.w * inv);
+        *reinterpret_cast<uint2*>((T*)P.out + ((int64_t)plan.x + r) * D + c) = packed;
+      }
     }
-    const float inv = 1.f / l;
-    *reinterpret_cast<uint32_t*>((T*)P.out + ((int64_t)plan.x + r) * D + c) = pack2<T>(x * inv, y * inv);
   }
 }
 
@@ -521,7 +594,7 @@ int launch_paged_attention(AttnParams P, cudaStream_t s) {
   BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, NB, ALIGNED>, dim3(grid), dim3(kThreads), smem, s, P));
   if (int rc = check_launch("paged_attention_kernel")) return rc;
   if (P.whole) return BSB_OK;
-  BSB_CUDA(launch_pdl(paged_attention_join_kernel<T, D>, dim3(grid), dim3(256), 0, s, P));
+  BSB_CUDA(launch_pdl(paged_attention_join_kernel<T, D>, dim3(grid), dim3(kJoinThreads), 0, s, P));
   return check_launch("paged_attention_join_kernel");
 }
 template <typename T, int D>
@@ -541,7 +614,7 @@ extern "C" {
 int64_t bsb_paged_attention_scratch_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (batch < 0 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || q_heads % kv_heads != 0) return -1;
   const int rows = q_heads / kv_heads < kRows ? q_heads / kv_heads : kRows;
-  return (int64_t)sm_count() * kMaxCtas * (16 + 2 * (2 * kRows + (int64_t)rows * head_dim) * 4);
+  return (int64_t)sm_count() * kMaxCtas * (32 + 2 * (2 * kRows + (int64_t)rows * head_dim) * 4);
 }
 
 int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -598,7 +671,7 @@ int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int6
   P.page_size = page_size;
   P.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   P.plan = reinterpret_cast<int4*>(scratch);
-  P.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)sm_count() * kMaxCtas * 16);
+  P.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)sm_count() * kMaxCtas * 32);
   // more requests than a launch keeps prefix sums of: launch after launch, in stream order, on the same scratch
   for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatch) {
     P.batch = batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch;
