@@ -33,7 +33,7 @@ constexpr int kBins = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxPart = 32768;                 // tokens of one CTA: 2^15 limbs of 17 bits add up below 2^32
 constexpr int kMaxVocab = kMaxCluster * kMaxPart;
-constexpr int kList = 256;                      // tokens that are compared with one another
+constexpr int kList = 128;                      // tokens that are compared with one another (256: 64 mixed rows 71 us instead of 60)
 constexpr float kSpan = 32.f;                   // the histogram's steps cover this many temperatures below the maximum
 
 // values in shared memory: the logits' own type, NaN as -infinity
@@ -57,8 +57,8 @@ struct Weigher {
   uint32_t vanish;        // high word of the (negative) exponent from which on a weight is below half a unit
   int unit;               // S
   __device__ __forceinline__ uint64_t operator()(float x) const {
+    // No branch: callers take several values side by side, and the chain of 64-bit operations is long.
     const double t = ((double)x - top) * c256;    // (never NaN: infinite maxima were mapped away, and c256 > 0)
-    if ((uint32_t)__double2hiint(t) >= vanish) return 0;
     const double magic = 6755399441055744.0;      // 1.5 * 2^52: adding it leaves the nearest integer in the low word
     const double s = t + magic;
     const double r = t - (s - magic);             // at most a half, in 256ths
@@ -70,7 +70,8 @@ struct Weigher {
     p = fma(r, p, 1.0);
     const double w = powers[i & 255] * p;         // times 2^(S + i / 256), by its exponent
     const double scaled = __hiloint2double(__double2hiint(w) + ((i >> 8) + unit) * (1 << 20), __double2loint(w));
-    return (uint64_t)__double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // rounded to a whole number of units
+    const uint64_t rounded = (uint64_t)__double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // a whole number of units
+    return (uint32_t)__double2hiint(t) >= vanish ? 0 : rounded;
   }
 };
 
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 
   const float mp = P.min_p ? P.min_p[b] : 0.f;
   const double least = mp > 0.f ? (double)fminf(mp, 1.f) * (double)(1ull << P.unit) : 0.0;   // the likeliest token always stays
+  const uint64_t fewest = (uint64_t)ceil(least);   // units of a token that stays
   const double u = P.uniforms[b] > 0.f ? (double)fminf(P.uniforms[b], 0.99999994f) : 0.0;
   auto chosen = [&](int64_t token, float x, uint64_t total) {
     P.tokens[b] = token;
@@ -286,17 +288,48 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       if (round > 0) row_sync();                 // (every CTA has read the histograms of the round before)
       for (int i = tid; i < kBins; i += kSampleThreads) reinterpret_cast<uint4*>(&S.hist[0][0])[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
-      each([&](float x) {
-        if (x < cut.x || (round > 0 && !inside(x))) return;
-        const int q = bin_of(x);
-        atomicAdd(&S.hist[0][q], 1u);
-        if (by_mass && x > cut.x) {              // (the share of the ties that a top-k cut leaves is added below, once)
-          const uint64_t w = weigh(x);
-          atomicAdd(&S.hist[1][q], (uint32_t)w & 0x1FFFFu);
-          atomicAdd(&S.hist[2][q], (uint32_t)(w >> 17) & 0x1FFFFu);
-          atomicAdd(&S.hist[3][q], (uint32_t)(w >> 34));
-        }
-      });
+      auto add_mass = [&](int q, uint64_t w) {
+        atomicAdd(&S.hist[1][q], (uint32_t)w & 0x1FFFFu);
+        atomicAdd(&S.hist[2][q], (uint32_t)(w >> 17) & 0x1FFFFu);
+        atomicAdd(&S.hist[3][q], (uint32_t)(w >> 34));
+      };
+      // (the share of the ties that a top-k cut leaves is added below, once: only what lies above the cut has its weight added)
+      if (round == 0 && !by_mass) {
+        each([&](float x) { atomicAdd(&S.hist[0][whole(step_of(x))], 1u); });
+      } else if (round == 0) {
+        each_vec([&](const T* v, int) {
+#pragma unroll
+          for (int e0 = 0; e0 < kPer; e0 += 4) {  // four values side by side: a weight is a long chain of 64-bit operations
+            uint64_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = weigh(to_f(v[e0 + e]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = to_f(v[e0 + e]);
+              if (x < cut.x) continue;
+              const int q = whole(step_of(x));
+              atomicAdd(&S.hist[0][q], 1u);
+              if (x > cut.x) add_mass(q, w[e]);
+            }
+          }
+        });
+      } else {                                   // few tokens are inside the bins chosen so far
+        each_vec([&](const T* v, int at) {
+          uint32_t in = 0;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const float x = to_f(v[e]);
+            in |= (x >= cut.x && whole(step_of(x)) == coarse ? 1u : 0u) << e;
+          }
+          for (; in != 0; in &= in - 1) {
+            const float x = to_f(vals[at + __ffs(in) - 1]);
+            if (!inside(x)) continue;
+            const int q = bin_of(x);
+            atomicAdd(&S.hist[0][q], 1u);
+            if (by_mass && x > cut.x) add_mass(q, weigh(x));
+          }
+        });
+      }
       __syncthreads();
       if (by_mass && rank == 0 && tid == 0 && (round == 0 || inside(cut.x))) {
         const int q = bin_of(cut.x);
@@ -307,19 +340,25 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       }
       row_sync();
       // every CTA adds up all bins of the row and scans them
-      constexpr int kEach = kBins / kSampleThreads;
-      uint64_t m[kEach], um = 0;
-      uint32_t c[kEach], uc = 0;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        m[i] = 0;
-        c[i] = 0;
+      constexpr int kEach = 4;                   // (16-byte loads from the peers, by half the threads)
+      uint64_t m[kEach] = {0, 0, 0, 0}, um = 0;
+      uint32_t c[kEach] = {0, 0, 0, 0}, uc = 0;
+      if (tid < kBins / kEach)
         for (int peer = 0; peer < C; ++peer) {
           const SampleShared* o = cluster.map_shared_rank(&S, peer);
-          const int q = tid * kEach + i;
-          c[i] += o->hist[0][q];
-          if (by_mass) m[i] += (uint64_t)o->hist[1][q] + ((uint64_t)o->hist[2][q] << 17) + ((uint64_t)o->hist[3][q] << 34);
+          uint4 part[4];
+#pragma unroll
+          for (int l = 0; l < 4; ++l)
+            part[l] = l == 0 || by_mass ? *reinterpret_cast<const uint4*>(&o->hist[l][tid * kEach]) : make_uint4(0, 0, 0, 0);
+          const uint32_t* word = reinterpret_cast<const uint32_t*>(part);
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            c[i] += word[i];
+            m[i] += (uint64_t)word[4 + i] + ((uint64_t)word[8 + i] << 17) + ((uint64_t)word[12 + i] << 34);
+          }
         }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
         um += m[i];
         uc += c[i];
       }
@@ -345,7 +384,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         const double upto = by_mass ? (double)(um + m[i]) : (double)(uc + c[i]), from = by_mass ? (double)um : (double)uc;
-        if (upto >= want && from < want) S.found = Found{um, m[i], want, uc, c[i], tid * kEach + i};
+        if (tid < kBins / kEach && upto >= want && from < want) S.found = Found{um, m[i], want, uc, c[i], tid * kEach + i};
         um += m[i];
         uc += c[i];
       }
@@ -381,15 +420,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     if (tid == 0) S.own_listed = 0;
     __syncthreads();
     each_vec([&](const T* v, int at) {
+      uint32_t in = 0;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         const float x = to_f(v[e]);
-        if (x >= cut.x && (all ? whole(step_of(x)) <= coarse : inside(x))) {
-          const uint32_t i = atomicAdd(&S.own_listed, 1u);
-          if (i < kList) {
-            S.own_x[i] = x;
-            S.own_at[i] = (uint32_t)(base + at + e);
-          }
+        const int q = whole(step_of(x));
+        in |= (x >= cut.x && (all ? q <= coarse : q == coarse) ? 1u : 0u) << e;
+      }
+      for (; in != 0; in &= in - 1) {
+        const int e = __ffs(in) - 1;
+        const float x = to_f(vals[at + e]);
+        if (!all && !inside(x)) continue;
+        const uint32_t i = atomicAdd(&S.own_listed, 1u);
+        if (i < kList) {
+          S.own_x[i] = x;
+          S.own_at[i] = (uint32_t)(base + at + e);
         }
       }
     });
@@ -418,14 +463,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       const uint64_t w = mine ? S.list_w[i] : 0;
       uint32_t higher = 0, equal = 0, first = 0;
       uint64_t heavier = 0;
-      if (mine)
-        for (int j = sub; j < size; j += lanes) {
-          const float other = S.list_x[j];
-          higher += other > x;
-          equal += other == x;
-          first += other == x && S.list_at[j] < at;
-          heavier += other > x ? S.list_w[j] : 0;
+      if (mine) {
+        if (all) {
+#pragma unroll 4
+          for (int j = sub; j < size; j += lanes) {
+            const float other = S.list_x[j];
+            higher += other > x;
+            equal += other == x;
+            first += other == x && S.list_at[j] < at;
+          }
+        } else {
+#pragma unroll 4
+          for (int j = sub; j < size; j += lanes) {
+            const float other = S.list_x[j];
+            higher += other > x;
+            equal += other == x;
+          }
         }
+        if (by_mass || (all && p < 1.f)) {
+#pragma unroll 4
+          for (int j = sub; j < size; j += lanes) heavier += S.list_x[j] > x ? S.list_w[j] : 0;
+        }
+      }
       for (int o = 1; o < lanes; o <<= 1) {
         higher += __shfl_xor_sync(0xFFFFFFFFu, higher, o);
         equal += __shfl_xor_sync(0xFFFFFFFFu, equal, o);
@@ -461,7 +520,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       }
       const Cut c = S.ex.cut;
       if (all) {                                 // the draw, among the listed
-        const bool keep = mine && (x > c.x || (x == c.x && first < c.ties)) && (double)w >= least;
+        const bool keep = mine && (x > c.x || (x == c.x && first < c.ties)) && w >= fewest;
         if (mine && sub == 0) S.list_w[i] = keep ? w : 0;
         __syncthreads();
         uint64_t before = 0, total = 0;
@@ -528,39 +587,59 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     __syncthreads();
   }
-  auto run_weights = [&](int r, float (&x)[8], uint64_t (&w)[8]) {
+  auto kept_of = [&](int r, float (&x)[8]) {      // this lane's values of a run, and which of them are kept
     run_vals(r, x);
-    uint32_t tie_rank = 0;
-    if (cut.partial) {
-      uint32_t own = 0;
+    uint32_t keep = 0;
+    if (!cut.partial) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) own += x[e] == cut.x;
-      uint32_t upto = own;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += y;
-      }
-      tie_rank = S.run_ties[r] + upto - own;
+      for (int e = 0; e < 8; ++e) keep |= (x[e] > cut.x || x[e] == cut.x ? 1u : 0u) << e;
+      return keep;
     }
-    uint64_t sum = 0;
+    uint32_t own = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) own += x[e] == cut.x;
+    uint32_t upto = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    uint32_t tie_rank = S.run_ties[r] + upto - own;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool tie = x[e] == cut.x;
-      w[e] = 0;
-      if (x[e] > cut.x || (tie && (!cut.partial || tie_rank < cut.ties))) {
-        w[e] = weigh(x[e]);
-        if (least > 0.0 && (double)w[e] < least) w[e] = 0;
-      }
+      keep |= (x[e] > cut.x || (tie && tie_rank < cut.ties) ? 1u : 0u) << e;
       tie_rank += tie;
-      sum += w[e];
+    }
+    return keep;
+  };
+  auto run_weights = [&](const float (&x)[8], uint32_t keep, uint64_t (&w)[8]) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e0 = 0; e0 < 8; e0 += 4) {
+#pragma unroll
+      for (int e = e0; e < e0 + 4; ++e) w[e] = weigh(x[e]);
+#pragma unroll
+      for (int e = e0; e < e0 + 4; ++e) {
+        if (!(keep >> e & 1) || w[e] < fewest) w[e] = 0;
+        sum += w[e];
+      }
     }
     return sum;
   };
   uint64_t mine = 0;
   for (int r = warp; r < runs; r += kSampleWarps) {
     float x[8];
-    uint64_t w[8];
-    uint64_t sum = run_weights(r, x, w);
+    uint32_t keep = kept_of(r, x);
+    uint64_t sum = 0;
+    if (__reduce_max_sync(0xFFFFFFFFu, __popc(keep)) > 2) {
+      uint64_t w[8];
+      sum = run_weights(x, keep, w);
+    } else {                                     // few are: one after the other is shorter than all side by side
+      for (; keep != 0; keep &= keep - 1) {
+        const uint64_t w = weigh(to_f(vals[r * kRun + lane * 8 + __ffs(keep) - 1]));
+        sum += w < fewest ? 0 : w;
+      }
+    }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) S.run_mass[r] = sum;
     mine += sum;
@@ -591,7 +670,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (run < 0) return;
   float x[8];
   uint64_t w[8];
-  const uint64_t sum = run_weights(run, x, w);
+  const uint32_t keep = kept_of(run, x);
+  const uint64_t sum = run_weights(x, keep, w);
   uint64_t upto = sum;
   for (int o = 1; o < 32; o <<= 1) {
     const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
