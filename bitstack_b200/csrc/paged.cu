@@ -170,9 +170,11 @@ __global__ void __launch_bounds__(kTableThreads) release_pages_kernel(const uint
 }
 
 // One CTA per token; a thread takes eight pairs (i, i + D/2) of a head: two 16-byte loads, two 16-byte stores, and the
-// token's cosines and sines from L1.  Bound by the copy: every byte of q, k and v is read once and written once.
+// token's cosines and sines from L1.  Bound by the copy: every byte of q, k and v is read once and written once.  The values
+// are asked for in front of the token's position, which the table rows and the destination wait for.
+constexpr int kRopeThreads = 512;   // at most; the launch takes as many as give every thread the same number of items
 template <typename T>
-__global__ void __launch_bounds__(256) rope_paged_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+__global__ void __launch_bounds__(kRopeThreads) rope_paged_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                                                          int64_t q_stride, int64_t k_stride, int64_t v_stride, const T* __restrict__ cos_t,
                                                          const T* __restrict__ sin_t, int64_t table_len, const int64_t* __restrict__ positions,
                                                          const int64_t* __restrict__ slots, T* __restrict__ q_out, T* __restrict__ k_pages,
@@ -180,34 +182,34 @@ __global__ void __launch_bounds__(256) rope_paged_kernel(const T* __restrict__ q
                                                          int64_t v_page_stride, int Hq, int Hkv, int D, int page_size, int* __restrict__ status) {
   pdl_enter();
   const int64_t t = blockIdx.x;
-  const int64_t pos = positions[t], slot = slots[t];
-  const bool bad = pos >= table_len || slot >= num_pages * page_size;
-  if (bad && threadIdx.x == 0) atomicCAS(status, 0, 62);
-  const bool turn = pos >= 0 && pos < table_len, keep = slot >= 0 && slot < num_pages * page_size && turn;
-  const int64_t page = keep ? slot / page_size : 0, row = keep ? slot % page_size : 0;
   const int parts = D / 16, items = (Hq + 2 * Hkv) * parts;
-  const float nan = __int_as_float(0x7FC00000);
   for (int it = threadIdx.x; it < items; it += blockDim.x) {
     const int head = it / parts, c = (it - head * parts) * 8;
+    const T* src = head < Hq         ? q + t * q_stride + (int64_t)head * D + c
+                   : head < Hq + Hkv ? k + t * k_stride + (int64_t)(head - Hq) * D + c
+                                     : v + t * v_stride + (int64_t)(head - Hq - Hkv) * D + c;
+    const uint4 lo = __ldcs(reinterpret_cast<const uint4*>(src)), hi = __ldcs(reinterpret_cast<const uint4*>(src + D / 2));
+    const int64_t pos = positions[t], slot = slots[t];
+    const bool bad = pos >= table_len || slot >= num_pages * page_size;
+    if (bad && it == 0) atomicCAS(status, 0, 62);
+    const bool turn = pos >= 0 && pos < table_len, keep = slot >= 0 && slot < num_pages * page_size && turn;
     if (head >= Hq && !keep) continue;
+    const int64_t page = keep ? slot / page_size : 0, row = keep ? slot % page_size : 0;
     if (head >= Hq + Hkv) {   // v: copied
-      const int h = head - Hq - Hkv;
-      const T* src = v + t * v_stride + (int64_t)h * D + c;
-      T* dst = v_pages + page * v_page_stride + ((int64_t)h * page_size + row) * D + c;
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-      *reinterpret_cast<uint4*>(dst + D / 2) = *reinterpret_cast<const uint4*>(src + D / 2);
+      T* dst = v_pages + page * v_page_stride + ((int64_t)(head - Hq - Hkv) * page_size + row) * D + c;
+      *reinterpret_cast<uint4*>(dst) = lo;
+      *reinterpret_cast<uint4*>(dst + D / 2) = hi;
       continue;
     }
     float a[8], b[8];
     if (turn) {
-      const T* src = head < Hq ? q + t * q_stride + (int64_t)head * D + c : k + t * k_stride + (int64_t)(head - Hq) * D + c;
       float c0[8], c1[8], s0[8], s1[8];
-      load8(src, a);
-      load8(src + D / 2, b);
       load8(cos_t + pos * D + c, c0);
       load8(cos_t + pos * D + c + D / 2, c1);
       load8(sin_t + pos * D + c, s0);
       load8(sin_t + pos * D + c + D / 2, s1);
+      unpack8<T>(lo, a);
+      unpack8<T>(hi, b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float x0 = a[e], x1 = b[e];   // x*cos + rotate_half(x)*sin with rotate_half(x) = [-x1, x0]
@@ -215,8 +217,9 @@ __global__ void __launch_bounds__(256) rope_paged_kernel(const T* __restrict__ q
         b[e] = x1 * c1[e] + x0 * s1[e];
       }
     } else {
+      const float fill = bad ? __int_as_float(0x7FC00000) : 0.f;   // padding: zeros; a position behind the tables: NaN
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] = b[e] = bad ? nan : 0.f;   // padding: zeros; a position behind the tables: NaN
+      for (int e = 0; e < 8; ++e) a[e] = b[e] = fill;
     }
     T* dst = head < Hq ? q_out + (t * Hq + head) * (int64_t)D + c
                        : k_pages + page * k_page_stride + ((int64_t)(head - Hq) * page_size + row) * D + c;
@@ -294,13 +297,15 @@ int bsb_rope_paged_cache(const void* q, const void* k, const void* v, int64_t q_
   int* status = device_status_word();
   if (status == nullptr) return BSB_ECUDA;
   const dim3 grid((unsigned)tokens);
+  const int64_t items = ((int64_t)q_heads + 2 * (int64_t)kv_heads) * (head_dim / 16), trips = ceil_div64(items, kRopeThreads);
+  const dim3 block((unsigned)(ceil_div64(ceil_div64(items, trips), 32) * 32));
   if (dtype == BSB_F16)
-    BSB_CUDA(launch_pdl(rope_paged_kernel<__half>, grid, dim3(256), 0, (cudaStream_t)stream, (const __half*)q, (const __half*)k, (const __half*)v,
+    BSB_CUDA(launch_pdl(rope_paged_kernel<__half>, grid, block, 0, (cudaStream_t)stream, (const __half*)q, (const __half*)k, (const __half*)v,
                         q_stride, k_stride, v_stride, (const __half*)cos_table, (const __half*)sin_table, table_len, positions, slots,
                         (__half*)q_out, (__half*)k_pages, (__half*)v_pages, num_pages, k_page_stride, v_page_stride, q_heads, kv_heads,
                         head_dim, page_size, status));
   else
-    BSB_CUDA(launch_pdl(rope_paged_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k,
+    BSB_CUDA(launch_pdl(rope_paged_kernel<__nv_bfloat16>, grid, block, 0, (cudaStream_t)stream, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k,
                         (const __nv_bfloat16*)v, q_stride, k_stride, v_stride, (const __nv_bfloat16*)cos_table, (const __nv_bfloat16*)sin_table,
                         table_len, positions, slots, (__nv_bfloat16*)q_out, (__nv_bfloat16*)k_pages, (__nv_bfloat16*)v_pages, num_pages,
                         k_page_stride, v_page_stride, q_heads, kv_heads, head_dim, page_size, status));
