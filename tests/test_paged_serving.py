@@ -459,3 +459,82 @@ def test_sample_step_frequencies():
     tokens = torch.zeros(n, dtype=torch.int64, device=DEV)
     glue.sample_step(x.repeat(n, 1), u, tokens)
     assert bool(((tokens.bincount(minlength=V) - torch.softmax(x[0].double(), 0) * n).abs() <= 1.0001).all())
+
+
+# ------------------------------------------------------------------------------------------------ calls side by side
+
+def test_more_requests_than_one_launch_takes():
+    """4100 requests: three launches on one scratch, idle rows and one-token requests among them."""
+    g = _gen(4, 1, 0, 0)
+    lens = torch.randint(0, 40, (4100,), generator=torch.Generator().manual_seed(4)).tolist()
+    hq, hkv, d, ps, dtype = 2, 1, 64, 16, torch.float16
+    kp, vp, table = _make_requests(lens, hkv, ps, d, dtype, g, poison=False)
+    table = torch.cat([table, torch.full((4100, 40), -1, dtype=torch.int32, device=DEV)], 1)   # wide enough for the shared form
+    q, k, v = _qkv_rows(4100, hq, hkv, d, dtype, g, False)
+    cos, sin = _tables_of_rotary(41, d, dtype)
+    out = glue.paged_decode_attention(q, k, v, cos, sin, torch.tensor([n - 1 for n in lens], device=DEV), table, kp, vp, hq, hkv, d)
+    some = list(range(0, 4100, 97)) + [2047, 2048, 4095, 4096, 4099]
+    at = torch.tensor(some, device=DEV)
+    _check_attention(out[at], q[at], k[at], v[at], cos, sin, [lens[i] for i in some], table[at], kp, vp, hq, hkv, d, ps, dtype)
+
+
+def test_calls_on_several_streams_at_once():
+    """Attention and sampling on four streams at the same time, each with scratch of its own: the results of one after the other."""
+    jobs = []
+    for i in range(4):
+        g = _gen(9, i)
+        lens, hq, hkv, d, ps, dtype = [900 + 100 * i, 40, 0, 613], 8, 2, 128, 16, torch.float16
+        kp, vp, table = _make_requests(lens, hkv, ps, d, dtype, g)
+        q, k, v = _qkv_rows(4, hq, hkv, d, dtype, g, False)
+        cos, sin = _tables_of_rotary(1300, d, dtype)
+        pos = torch.tensor([n - 1 for n in lens], device=DEV)
+        logits = torch.randn(5, 30000, device=DEV, generator=g)
+        u, p = torch.rand(5, device=DEV, generator=g), torch.full((5,), 0.9, device=DEV)
+        jobs.append((q, k, v, cos, sin, pos, table, kp, vp, hq, hkv, d, logits, u, p))
+
+    def run(j):
+        return (glue.paged_decode_attention(*j[:12]), glue.sample_step(j[12], j[13], torch.zeros(5, dtype=torch.int64, device=DEV), top_p=j[14]))
+    want = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in jobs], [[] for _ in jobs]
+    for _ in range(20):
+        for i, (j, s) in enumerate(zip(jobs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(run(j))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(a, b) for r in gs for a, b in zip(r, w))
+
+
+def test_table_rows_that_several_requests_share():
+    """A common prefix: pages that two requests' rows both list are read by both (each writes a page of its own)."""
+    g, hq, hkv, d, ps, dtype = _gen(3, 3), 4, 2, 64, 8, torch.float16
+    kp, vp = _pool(12, hkv, ps, d, dtype, g, False)
+    table = torch.tensor([[3, 5, 7, 1], [3, 5, 7, 2], [3, 5, 7, 9]], dtype=torch.int32, device=DEV)
+    q, k, v = _qkv_rows(3, hq, hkv, d, dtype, g, False)
+    cos, sin = _tables_of_rotary(32, d, dtype)
+    lens = [25, 30, 32]
+    out = glue.paged_decode_attention(q, k, v, cos, sin, torch.tensor([n - 1 for n in lens], device=DEV), table, kp, vp, hq, hkv, d)
+    _check_attention(out, q, k, v, cos, sin, lens, table, kp, vp, hq, hkv, d, ps, dtype)
+
+
+def test_wrong_arguments_on_the_device():
+    x = torch.zeros(2, 128, device=DEV, dtype=torch.float16)
+    pool, i = torch.zeros(4, 1, 8, 128, device=DEV, dtype=torch.float16), torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    pos = torch.full((2,), -1, device=DEV)
+    ok = dict(q=x, k=x, v=x, cos=x, sin=x, positions=pos, block_table=i, k_pages=pool, v_pages=pool, q_heads=1, kv_heads=1, head_dim=128)
+    assert bool((glue.paged_decode_attention(**ok) == 0).all())
+    for bad in (dict(k=x[:1]), dict(v=x.bfloat16()), dict(positions=pos.int()), dict(block_table=i.long()), dict(block_table=i[:1]), dict(cos=x[:, :64]),
+                dict(k_pages=pool[:, :, :, :64]), dict(v_pages=pool[:3]), dict(k_pages=pool.transpose(0, 2)), dict(q=x.t()), dict(q_heads=2),
+                dict(k_pages=pool.expand(4, 1, 8, 128)[:, :, :0]), dict(k_pages=pool[:1].expand(4, 1, 8, 128)), dict(positions=pos.cpu()), dict(kv_heads=0)):
+        with pytest.raises(ValueError):
+            glue.paged_decode_attention(**{**ok, **bad})
+    lo, u, t = torch.zeros(2, 9, device=DEV), torch.zeros(2, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+    for bad in (dict(uniforms=u[:1]), dict(tokens=t.int()), dict(temperature=u.double()), dict(top_k=u), dict(top_p=u[:1]), dict(pos=t), dict(logits=lo.t()),
+                dict(logits=lo[:1].expand(2, 9)), dict(logprobs=u.cpu())):
+        with pytest.raises(ValueError):
+            glue.sample_step(**{**dict(logits=lo, uniforms=u, tokens=t), **bad})
+    n, c = torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    for bad in (dict(page_size=0), dict(page_size=1 << 40), dict(max_tokens=-1), dict(free_count=n), dict(lens_out=c), dict(new_tokens=n.long()), dict(free_pages=c[:0])):
+        with pytest.raises(ValueError):
+            glue.page_tables(**{**dict(lens=n, new_tokens=n, block_table=i, free_pages=c, free_count=c, page_size=4), **bad})
