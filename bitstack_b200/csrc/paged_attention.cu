@@ -12,9 +12,10 @@
 //  * All query heads of a group share the K and V that were read.  The products are taken transposed, scores^T = K Q^T and
 //    output^T = V^T P^T, so that positions and dimensions fill the 16 rows of mma.sync m16n8k16 and the heads its 8 columns: a
 //    group of up to 8 heads wastes nothing (half the MMAs, exponentials and accumulators of the untransposed form), one of up
-//    to 16 takes two column blocks.  Scores and output are accumulated in fp32, the weights are rounded to the cache's type for
-//    the second product (half a step of relative error each, as q is rounded after its rotation), and one pass keeps the
-//    running maximum and sum.
+//    to 16 takes two column blocks.  q after its rotation and the weights go in as two values of the type each, the nearest one
+//    and what that leaves: twice the MMAs, 1.5 % of the time (118 -> 119 us, 64 requests), and the only rounding that is left is
+//    the output's (without: twice its error).  Scores and output are accumulated in fp32; one pass keeps the running maximum
+//    and sum.
 //  * The new position's K and V come from the projection's output: turned, stored to the page and to the ring by the warp
 //    that meets the position, so nothing is read back.
 #include <climits>
@@ -73,10 +74,10 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<T, __half>)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // an 8 x 8 block of 16-bit values across the warp
@@ -107,6 +108,31 @@ __device__ __forceinline__ int length_of(const AttnParams& P, int b) {
 }
 __device__ __forceinline__ int tiles_of(int n) { return n <= 0 ? 1 : (n + kTile - 1) / kTile; }   // idle rows too have an output
 
+// four values of the type as fp32; and back, leaving in x what the rounding took
+template <typename T>
+__device__ __forceinline__ void load4(const T* src, float (&x)[4]) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(src);
+  const typename Pair<T>::type* p = reinterpret_cast<const typename Pair<T>::type*>(&raw);
+  const float2 a = to_f2(p[0]), b = to_f2(p[1]);
+  x[0] = a.x;
+  x[1] = a.y;
+  x[2] = b.x;
+  x[3] = b.y;
+}
+template <typename T>
+__device__ __forceinline__ void store4(uint8_t* dst, float (&x)[4]) {
+  uint2 raw;
+  typename Pair<T>::type* p = reinterpret_cast<typename Pair<T>::type*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    p[i] = Pair<T>::make(x[2 * i], x[2 * i + 1]);
+    const float2 f = to_f2(p[i]);
+    x[2 * i] -= f.x;
+    x[2 * i + 1] -= f.y;
+  }
+  *reinterpret_cast<uint2*>(dst) = raw;
+}
+
 // rotary embedding of eight pairs (i, i + D/2): x*cos + rotate_half(x)*sin with rotate_half(x) = [-x1, x0]
 template <typename T, int D>
 __device__ __forceinline__ void turn8(const T* src, const T* cos_t, const T* sin_t, float (&x0)[8], float (&x1)[8]) {
@@ -127,7 +153,7 @@ __device__ __forceinline__ void turn8(const T* src, const T* cos_t, const T* sin
 
 // dynamic shared memory: [warp][stage][K 16 rows, V 16 rows], q [16 rows], maxima and sums [2][warp][16], prefix sums [batch + 1]
 template <int D> constexpr int ring_bytes() { return kWarps * Shape<D>::stages * 2 * 16 * D * 2; }
-template <int D> constexpr int fixed_bytes() { return ring_bytes<D>() + kRows * D * 2 + 2 * kWarps * kRows * 4; }
+template <int D> constexpr int fixed_bytes() { return ring_bytes<D>() + 2 * kRows * D * 2 + 2 * kWarps * kRows * 4; }
 
 // NB: column blocks of 8 heads.  ALIGNED: pages are a multiple of 16 rows, so the 16 positions of a warp lie in one page.
 template <typename T, int D, int NB, bool ALIGNED>
@@ -138,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
   constexpr int kHalf = 16 * D * 2;              // bytes of the K (or V) rows of a stage
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* s_q = smem + ring_bytes<D>();
-  float* s_m = reinterpret_cast<float*>(s_q + kRows * D * 2);
+  float* s_m = reinterpret_cast<float*>(s_q + 2 * kRows * D * 2);
   float* s_l = s_m + kWarps * kRows;
   int64_t* s_before = reinterpret_cast<int64_t*>(s_l + kWarps * kRows);
   __shared__ int64_t s_sum[kWarps];
@@ -311,19 +337,34 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     cp_async_commit();
   };
 
-  // ---- q: turned, rounded to the type, rows behind the group zero ------------------------------------------------
+  // ---- q: turned, as the type's nearest value and what that leaves (the products see q as exactly as fp32 does); rows behind the
+  // group zero.  A thread takes four pairs (i, i + D/2).
   auto stage_q = [&]() {
-    for (int it = tid; it < NB * 8 * (D / 16); it += kThreads) {
-      const int r = it / (D / 16), c = it - r * (D / 16);
-      float x0[8], x1[8];
+    for (int it = tid; it < NB * 8 * (D / 8); it += kThreads) {
+      const int r = it / (D / 8), c = (it - r * (D / 8)) * 4;
+      float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
       if (r < heads && n > 0) {
-        turn8<T, D>((const T*)P.q + b * P.q_stride + (int64_t)(head0 + r) * D + c * 8, cos_t + c * 8, sin_t + c * 8, x0, x1);
-      } else {
+        const T* src = (const T*)P.q + b * P.q_stride + (int64_t)(head0 + r) * D + c;
+        float a0[4], a1[4], c0[4], c1[4], s0[4], s1[4];
+        load4(src, a0);
+        load4(src + D / 2, a1);
+        load4(cos_t + c, c0);
+        load4(cos_t + c + D / 2, c1);
+        load4(sin_t + c, s0);
+        load4(sin_t + c + D / 2, s1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
+        for (int e = 0; e < 4; ++e) {
+          x0[e] = a0[e] * c0[e] - a1[e] * s0[e];
+          x1[e] = a1[e] * c1[e] + a0[e] * s1[e];
+        }
       }
-      *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((c ^ (r & 7)) << 4)) = pack8<T>(x0);
-      *reinterpret_cast<uint4*>(s_q + r * D * 2 + (((c + D / 16) ^ (r & 7)) << 4)) = pack8<T>(x1);
+      const int at0 = (((c >> 3) ^ (r & 7)) << 4) + (c & 4) * 2, at1 = ((((c + D / 2) >> 3) ^ (r & 7)) << 4) + (c & 4) * 2;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint8_t* row = s_q + (part * kRows + r) * D * 2;
+        store4<T>(row + at0, x0);
+        store4<T>(row + at1, x1);
+      }
     }
   };
 
@@ -338,12 +379,15 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
   issue(kStages - 1);
 
   while (true) {
-    uint32_t qf[NB][D / 32][4];                   // columns = heads: two k steps per load
+    uint32_t qf[NB][D / 32][4], qr[NB][D / 32][4];   // columns = heads: two k steps per load; and what the rounding of q left
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
       const int r = h * 8 + (lane & 7);
 #pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks) ldsm4(smem_u32(s_q) + r * D * 2 + (((4 * ks + (lane >> 3)) ^ (r & 7)) << 4), qf[h][ks]);
+      for (int ks = 0; ks < D / 32; ++ks) {
+        ldsm4(smem_u32(s_q) + r * D * 2 + (((4 * ks + (lane >> 3)) ^ (r & 7)) << 4), qf[h][ks]);
+        ldsm4(smem_u32(s_q) + kRows * D * 2 + r * D * 2 + (((4 * ks + (lane >> 3)) ^ (r & 7)) << 4), qr[h][ks]);
+      }
     }
 
     // heads 8h + 2 t4 and + 1 of this lane: running maximum (of the raw scores) and sum; output^T, rows = dimensions
@@ -364,18 +408,25 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
       const int left = n - (base0 + i * kTile);   // positions of these 16 that exist, if positive
       if (left > 0) {
         const uint32_t stage = stage_of(i);
-        float s[NB][4];                           // (position gid, heads), (position gid + 8, heads)
+        float s[NB][4], s_rest[NB][4];            // (position gid, heads), (position gid + 8, heads)
 #pragma unroll
         for (int h = 0; h < NB; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[h][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[h][e] = s_rest[h][e] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t kf[4];
           ldsm4((k_frag + stage) ^ (ks << 5), kf);
 #pragma unroll
-          for (int h = 0; h < NB; ++h) mma16816<T>(s[h], kf, qf[h][ks / 2][(ks & 1) * 2], qf[h][ks / 2][(ks & 1) * 2 + 1]);
+          for (int h = 0; h < NB; ++h) {
+            mma16816<T>(s[h], kf, qf[h][ks / 2][(ks & 1) * 2], qf[h][ks / 2][(ks & 1) * 2 + 1]);
+            mma16816<T>(s_rest[h], kf, qr[h][ks / 2][(ks & 1) * 2], qr[h][ks / 2][(ks & 1) * 2 + 1]);
+          }
         }
+#pragma unroll
+        for (int h = 0; h < NB; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][e] += s_rest[h][e];   // (two chains of products, half as long)
         if (left < 16) {
 #pragma unroll
           for (int h = 0; h < NB; ++h) {
@@ -414,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
             }
           }
         }
-        uint32_t pf[NB][2];                       // weights^T: rows = positions, columns = heads
+        uint32_t pf[NB][2], pr[NB][2];            // weights^T, rows = positions, columns = heads; and what their rounding left
 #pragma unroll
         for (int h = 0; h < NB; ++h) {
           const float c0 = -m[h][0] * P.scale_log2, c1 = -m[h][1] * P.scale_log2;
@@ -424,15 +475,23 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
           s[h][3] = fast_exp2(fmaf(s[h][3], P.scale_log2, c1));
           l[h][0] += s[h][0] + s[h][2];
           l[h][1] += s[h][1] + s[h][3];
-          pf[h][0] = transpose8(pack2<T>(s[h][0], s[h][1]));
-          pf[h][1] = transpose8(pack2<T>(s[h][2], s[h][3]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t p = pack2<T>(s[h][2 * e], s[h][2 * e + 1]);
+            const float2 f = to_f2(*reinterpret_cast<const typename Pair<T>::type*>(&p));
+            pf[h][e] = transpose8(p);
+            pr[h][e] = transpose8(pack2<T>(s[h][2 * e] - f.x, s[h][2 * e + 1] - f.y));
+          }
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           uint32_t vf[4];
           ldsm4_t((v_frag + stage) ^ (j << 5), vf);
 #pragma unroll
-          for (int h = 0; h < NB; ++h) mma16816<T>(o[h][j], vf, pf[h][0], pf[h][1]);
+          for (int h = 0; h < NB; ++h) {
+            mma16816<T>(o[h][j], vf, pf[h][0], pf[h][1]);
+            mma16816<T>(o[h][j], vf, pr[h][0], pr[h][1]);
+          }
         }
       }
       __syncwarp();                               // every lane has read the stage before it is filled again
