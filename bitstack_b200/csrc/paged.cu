@@ -11,7 +11,9 @@ namespace {
 
 constexpr int kTableThreads = 1024;
 constexpr int kTableRows = 8192;         // requests of one call: their prefix sums stay in shared memory
-constexpr int64_t kTokensInOne = 4096;   // longer token lists are written by a second, wider launch
+// Longer token lists are written by a second, wider launch (64 requests, one launch against two: 355 tokens 4.5 / 5.7 us, 2148
+// tokens 6.6 / 6.0, 8547 tokens 12.2 / 6.4, 21872 tokens 24.6 / 6.8).
+constexpr int64_t kTokensInOne = 1536;
 
 // inclusive scan of two counters over the CTA; `tot` receives the totals
 __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t (*red)[2], int64_t& tot_a, int64_t& tot_b) {
@@ -67,7 +69,8 @@ __device__ __forceinline__ void token_entry(int64_t t, const int32_t* offsets, i
   positions[t] = pos;
 }
 
-// One CTA: the whole step is two scans over the requests and a scatter, all of it latency.  lens_out may be lens, and
+// One CTA: the whole step is two scans over the requests and a scatter, all of it latency (256 requests of one token: 4.8 us in a
+// graph, of which the launch is about half).  lens_out may be lens, and
 // free_count_out may be free_count: everything is read before the barriers in front of the writes.
 __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(
     const int32_t* lens, const int32_t* __restrict__ new_tokens, int batch, int32_t* __restrict__ table, int64_t table_stride,
@@ -170,8 +173,9 @@ __global__ void __launch_bounds__(kTableThreads) release_pages_kernel(const uint
 }
 
 // One CTA per token; a thread takes eight pairs (i, i + D/2) of a head: two 16-byte loads, two 16-byte stores, and the
-// token's cosines and sines from L1.  Bound by the copy: every byte of q, k and v is read once and written once.  The values
-// are asked for in front of the token's position, which the table rows and the destination wait for.
+// token's cosines and sines from L1.  Bound by the copy: every byte of q, k and v is read once and written once (2047 tokens of
+// 32 / 8 heads of 128: 10.9 us, 4.5 TB/s).  The values are asked for in front of the token's position, which the table rows and
+// the destination wait for, and every thread gets the same number of items (12.6 us with 256 threads and 1.5 items each).
 constexpr int kRopeThreads = 512;   // at most; the launch takes as many as give every thread the same number of items
 template <typename T>
 __global__ void __launch_bounds__(kRopeThreads) rope_paged_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,

@@ -1,7 +1,8 @@
 // One new token per request over a paged key/value cache: rotary embedding of q and k, k and v written into the request's
 // page, softmax(q K^T / sqrt(D)) V over the request's pages.
 //
-// Bound by reading K and V once (4 flops per byte and head of a group; the floor is their bytes at copy bandwidth).
+// Bound by reading K and V once (4 flops per byte and head of a group; the floor is their bytes at copy bandwidth).  Measured: 64
+// requests of 1 to 8192 positions, 32 / 8 heads of 128: 120 us, 6.0 TB/s (copy 6.55); one request of 131071: 90 us, 6.0 TB/s.
 //  * Work split: a request's length is cut into tiles of 64 positions; the tiles of all (request, kv head) pairs form one
 //    sequence, of which every CTA takes the same number.  Lengths are only known on the device, so every CTA finds its place
 //    by a prefix sum over the requests.  A pair that several CTAs share leaves partial results (maximum, sum, unnormalised
@@ -13,7 +14,7 @@
 //    output^T = V^T P^T, so that positions and dimensions fill the 16 rows of mma.sync m16n8k16 and the heads its 8 columns: a
 //    group of up to 8 heads wastes nothing (half the MMAs, exponentials and accumulators of the untransposed form), one of up
 //    to 16 takes two column blocks.  q after its rotation and the weights go in as two values of the type each, the nearest one
-//    and what that leaves: twice the MMAs, 1.5 % of the time (118 -> 119 us, 64 requests), and the only rounding that is left is
+//    and what that leaves: twice the MMAs, 1 % of the time (117 -> 118 us, 64 requests), and the only rounding that is left is
 //    the output's (without: twice its error).  Scores and output are accumulated in fp32; one pass keeps the running maximum
 //    and sum.
 //  * The new position's K and V come from the projection's output: turned, stored to the page and to the ring by the warp
@@ -31,10 +32,16 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16 * kWarps;       // positions of a tile
 constexpr int kRows = 16;                // most query heads of one pass
 constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix sums stay in shared memory
-constexpr int kPairCost = 3;             // what a pair costs a CTA beside its tiles, in tiles
+// What a pair costs a CTA beside its tiles, in tiles (64 ragged requests up to 8192 positions / 128 up to 1500, heads of 64: cost 0
+// 143 / 37 us, 1 126 / 29.5, 3 120 / 23.3, 6 120 / 25.4).
+constexpr int kPairCost = 3;
 constexpr float kSlack = 6.f;            // see the running maximum
-constexpr int64_t kWholePositions = 512; // requests that cannot be longer than this get one CTA per (request, kv head): no join
-template <int D> struct Shape;           // stages of a warp's ring, CTAs of a multiprocessor
+// Requests that cannot be longer than this get one CTA per (request, kv head) and no join.  32 / 8 heads of 128, one CTA per pair
+// against equal shares: 1 request of 200 6.5 / 8.0 us, of 512 9.2 / 8.1, of 1000 14.6 / 8.7; 16 requests of 512 9.4 / 10.9, of 1000
+// 14.7 / 12.0; 64 requests of 200 11.2 / 15.2.
+constexpr int64_t kWholePositions = 512;
+// Stages of a warp's ring, CTAs of a multiprocessor (64 ragged requests: 2 x 3 141 us, 3 x 2 147, 4 x 1 183, before the last steps).
+template <int D> struct Shape;
 template <> struct Shape<128> { static constexpr int stages = 2, ctas = 3; };
 template <> struct Shape<64> { static constexpr int stages = 3, ctas = 4; };
 constexpr int kMaxCtas = 4;              // per multiprocessor, for the scratch
