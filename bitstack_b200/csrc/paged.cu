@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_kernel(const T* __res
                                                          const int64_t* __restrict__ slots, T* __restrict__ q_out, T* __restrict__ k_pages,
                                                          T* __restrict__ v_pages, int64_t num_pages, int64_t k_page_stride,
                                                          int64_t v_page_stride, int Hq, int Hkv, int D, int page_size, int* __restrict__ status) {
-  pdl_enter();
+  pdl_wait();   // no early release: the dense decode attention reads older cache rows, which may be these pages, in front of its own wait
   const int64_t t = blockIdx.x;
   const int parts = D / 16, items = (Hq + 2 * Hkv) * parts;
   for (int it = threadIdx.x; it < items; it += blockDim.x) {

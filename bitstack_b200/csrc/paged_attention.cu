@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     if (!(begins && ends) && tid == 0)
       P.plan[2 * blockIdx.x + (begins ? 1 : 0)] = make_int4((int)out_row, done_heads, (int)divide(pair_begin, share), (int)divide(pair_end - 1, share));
     if (last) {
-      pdl_trigger();
+      if (!P.whole) pdl_trigger();                // (without a join, the next kernel starts when the new rows are in the pages)
       return;
     }
     stage_q();

@@ -40,6 +40,8 @@ class PagedDecoder:
         zeros = lambda *n, t: torch.zeros(*n, dtype=t, device=dev)  # noqa: E731
         width = -(-model.max_len // page_size)
         self.lens, self.active = zeros(rows, t=torch.int32), zeros(rows, t=torch.int32)
+        self.max_positions = width * page_size                 # of a request: whole pages
+        self.cos, self.sin = (model.cos, model.sin) if self.max_positions <= model.max_len else self._rotary(self.max_positions)
         self.block_table = torch.full((rows, width), -1, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev)     # the lowest page is on top
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=dev)
@@ -55,6 +57,12 @@ class PagedDecoder:
         self._running = [False] * rows                         # the host's view of which rows are taken
         self._graph = None
 
+    def _rotary(self, n):
+        s = self.model.shape
+        inv_freq = 1.0 / (s.rope_theta ** (torch.arange(0, s.head_dim, 2, device=self.device, dtype=torch.float32) / s.head_dim))
+        freqs = torch.outer(torch.arange(n, device=self.device, dtype=torch.float32), inv_freq)
+        return tuple(torch.cat([f, f], dim=-1).half() for f in (freqs.cos(), freqs.sin()))
+
     # ------------------------------------------------------------------ requests
     def free_rows(self) -> List[int]:
         return [i for i, busy in enumerate(self._running) if not busy]
@@ -68,8 +76,8 @@ class PagedDecoder:
         lengths = [int(p.numel()) for p in prompts]
         if not lengths or min(lengths) < 1:
             raise ValueError("a prompt must have at least one token")
-        if max(lengths) > self.model.max_len:
-            raise ValueError(f"a prompt of {max(lengths)} tokens is longer than the decoder's {self.model.max_len}")
+        if max(lengths) > self.max_positions:
+            raise ValueError(f"a prompt of {max(lengths)} tokens is longer than a request's {self.max_positions} positions")
         free = self.free_rows()
         if len(free) < len(prompts):
             raise OutOfPages(f"{len(prompts)} prompts, {len(free)} free rows")
@@ -82,13 +90,18 @@ class PagedDecoder:
         new[at] = torch.tensor(lengths, dtype=torch.int32, device=dev)
         self.temperature[at], self.top_k[at], self.top_p[at], self.min_p[at] = float(temperature), int(top_k), float(top_p), float(min_p)
         slots, positions, _, _ = glue.page_tables(self.lens, new, self.block_table, self.free_pages, self.free_count, self.page_size, total)
-        ids = torch.cat([p.reshape(-1) for p in prompts]).to(dev)
-        hidden = self._prompt(ids, slots, positions, lengths)
-        logits = hidden @ self.model.lm_head.t()
-        u = torch.rand(len(rows), device=dev) if uniforms is None else uniforms.to(dev, torch.float32)
-        drawn = torch.empty(len(rows), dtype=torch.int64, device=dev)
-        logprobs = torch.empty(len(rows), dtype=torch.float32, device=dev)
-        glue.sample_step(logits, u, drawn, self.temperature[at], self.top_k[at], self.top_p[at], self.min_p[at], logprobs=logprobs)
+        try:
+            ids = torch.cat([p.reshape(-1) for p in prompts]).to(dev)
+            hidden = self._prompt(ids, slots, positions, lengths)
+            logits = hidden @ self.model.lm_head.t()
+            u = torch.rand(len(rows), device=dev) if uniforms is None else uniforms.to(dev, torch.float32)
+            drawn = torch.empty(len(rows), dtype=torch.int64, device=dev)
+            logprobs = torch.empty(len(rows), dtype=torch.float32, device=dev)
+            glue.sample_step(logits, u, drawn, self.temperature[at], self.top_k[at], self.top_p[at], self.min_p[at], logprobs=logprobs)
+        except BaseException:                                  # the prompts' pages go back
+            done = new > 0
+            glue.release_pages(done, self.lens, self.block_table, self.free_pages, self.free_count, self.page_size)
+            raise
         self.tokens[at], self.logprobs[at], self.active[at] = drawn, logprobs, 1
         for r in rows:
             self._running[r] = True
@@ -117,7 +130,7 @@ class PagedDecoder:
         for i, lay in enumerate(m.layers):
             x = F.rms_norm(h, (s.hidden,), lay["in_norm"], s.rms_eps)
             q, k, v = forward_grouped([lay["self_attn.q_proj"], lay["self_attn.k_proj"], lay["self_attn.v_proj"]], x)
-            q = glue.rope_paged_cache(q, k, v, m.cos, m.sin, positions, slots, self.k_pages[i], self.v_pages[i], hq, hkv, hd)
+            q = glue.rope_paged_cache(q, k, v, self.cos, self.sin, positions, slots, self.k_pages[i], self.v_pages[i], hq, hkv, hd)
             keys, values = self.k_pages[i][page, :, row], self.v_pages[i][page, :, row]       # [tokens, kv heads, head_dim]
             att, lo = torch.empty_like(q), 0
             for n in lengths:
@@ -140,8 +153,8 @@ class PagedDecoder:
         for i, lay in enumerate(m.layers):
             x = glue.add_rmsnorm(h, delta, lay["in_norm"], s.rms_eps, absmax=am)
             q, k, v = forward_grouped([lay["self_attn.q_proj"], lay["self_attn.k_proj"], lay["self_attn.v_proj"]], x, x_absmax=am)
-            att = glue.paged_decode_attention(q, k, v, m.cos, m.sin, last, self.block_table, self.k_pages[i], self.v_pages[i], m.q_local,
-                                              m.kv_local, s.head_dim)
+            att = glue.paged_decode_attention(q, k, v, self.cos, self.sin, last, self.block_table, self.k_pages[i], self.v_pages[i],
+                                              m.q_local, m.kv_local, s.head_dim)
             x = glue.add_rmsnorm(h, lay["self_attn.o_proj"](att), lay["post_norm"], s.rms_eps, absmax=am)
             g, u = forward_grouped([lay["mlp.gate_proj"], lay["mlp.up_proj"]], x, x_absmax=am)
             a = glue.silu_mul(g, u, absmax=am)

@@ -191,7 +191,8 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  * position p of the request being row p % page_size of page block_table[b][p / page_size].  A SLOT is
  * page * page_size + row.  fp16 or bf16 (`dtype`: q, k, v, the cos / sin tables [table_len][head_dim], pages and output
  * alike), rows of q, k, v q_stride / k_stride / v_stride elements apart (multiples of 8), 16-byte aligned buffers.
- * An index that points outside its tensor is never followed: see bsb_read_status, codes 61-64.
+ * An index that points outside its tensor is never followed: see bsb_read_status, codes 61-64.  None of these calls lets the
+ * kernel behind it start before what it writes is there, so any other call may follow directly (bsb_decode_attention too).
  *
  * bsb_page_tables: one step of all requests.  Request b holds lens[b] tokens and gets new_tokens[b] more (negative counts
  *   are taken as 0).  Pages it lacks are popped from the stack free_pages[0 .. *free_count) (capacity entries), requests in

@@ -137,7 +137,32 @@ def test_pool_exhaustion(model):
     with pytest.raises(ValueError):
         d.submit([torch.zeros(0, dtype=torch.long)])
     with pytest.raises(ValueError):
-        d.submit(_prompts([129], 1))
+        d.submit(_prompts([d.max_positions + 1], 1))
+
+
+def test_a_request_up_to_its_last_position(model):
+    """128 positions in pages of 24: six whole pages, 144 positions; then the row makes no step, and nothing is NaN."""
+    from bitstack_b200 import _lib
+    from bitstack_b200.serving import PagedDecoder
+    d = PagedDecoder(model, rows=1, num_pages=8, page_size=24)
+    assert d.max_positions == 144
+    d.submit(_prompts([126], 1))
+    for n in range(126, 146):
+        d.step()
+        assert torch.isfinite(d.logits).all()
+        assert d.positions.tolist() == [n if n < 144 else -1]
+    _lib.check_device_status()
+    # the positions that the decoder's own tables hold are turned by the same numbers
+    assert torch.equal(d.cos[:128], model.cos) and torch.equal(d.sin[:128], model.sin)
+
+
+def test_a_prompt_that_fails_gives_its_pages_back(model, monkeypatch):
+    from bitstack_b200.serving import PagedDecoder
+    d = PagedDecoder(model, rows=2, num_pages=8, page_size=8)
+    monkeypatch.setattr(PagedDecoder, "_prompt", lambda self, *a: (_ for _ in ()).throw(RuntimeError("no")))
+    with pytest.raises(RuntimeError, match="no"):
+        d.submit(_prompts([20], 1))
+    assert int(d.free_count) == 8 and d.lens.tolist() == [0, 0] and d.free_rows() == [0, 1]
 
 
 def test_generate(model):

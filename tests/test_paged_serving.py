@@ -538,3 +538,26 @@ def test_wrong_arguments_on_the_device():
     for bad in (dict(page_size=0), dict(page_size=1 << 40), dict(max_tokens=-1), dict(free_count=n), dict(lens_out=c), dict(new_tokens=n.long()), dict(free_pages=c[:0])):
         with pytest.raises(ValueError):
             glue.page_tables(**{**dict(lens=n, new_tokens=n, block_table=i, free_pages=c, free_count=c, page_size=4), **bad})
+
+
+def test_pages_as_a_dense_cache():
+    """One page per request is the dense cache's layout: a prompt written by the paged call, then read by the dense decode
+    attention directly behind it, and the other way round."""
+    g, B, hq, hkv, d, L = _gen(11, 2), 3, 8, 2, 128, 700
+    cos, sin = _tables_of_rotary(L, d, torch.float16)
+    for _ in range(20):
+        kc, vc = (torch.zeros(B, hkv, L, d, device=DEV, dtype=torch.float16) for _ in range(2))
+        n = 650
+        q, k, v = _qkv_rows(B * n, hq, hkv, d, torch.float16, g, False)
+        pos = torch.arange(n, device=DEV).repeat(B)
+        slots = pos + torch.arange(B, device=DEV).repeat_interleave(n) * L
+        q1, k1, v1 = _qkv_rows(B, hq, hkv, d, torch.float16, g, False)
+        at = torch.tensor([n], device=DEV)
+        torch.cuda.synchronize()
+        glue.rope_paged_cache(q, k, v, cos, sin, pos, slots, kc, vc, hq, hkv, d)
+        dense = glue.decode_attention(q1, k1, v1, cos, sin, at, kc, vc, hq, hkv, d)
+        table = torch.arange(B, device=DEV, dtype=torch.int32).view(B, 1)
+        paged = glue.paged_decode_attention(q1, k1, v1, cos, sin, at.repeat(B), table, kc, vc, hq, hkv, d)
+        _check_attention(paged, q1, k1, v1, cos, sin, [n + 1] * B, table, kc, vc, hq, hkv, d, L, torch.float16)
+        # the dense call rounds q after its rotation too, accumulates in fp32 and sums 2^-18 off at most: the same bound
+        _check_attention(dense, q1, k1, v1, cos, sin, [n + 1] * B, table, kc, vc, hq, hkv, d, L, torch.float16)
