@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       // (the share of the ties that a top-k cut leaves is added below, once: only what lies above the cut has its weight added)
       if (round == 0 && !by_mass) {
         each([&](float x) { atomicAdd(&S.hist[0][whole(step_of(x))], 1u); });
-      } else if (round == 0) {
+      } else if (round == 0 && cut.x == -INFINITY) {
         each_vec([&](const T* v, int) {
 #pragma unroll
           for (int e0 = 0; e0 < kPer; e0 += 4) {  // four values side by side: a weight is a long chain of 64-bit operations
@@ -310,25 +310,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             for (int e = 0; e < 4; ++e) w[e] = weigh(to_f(v[e0 + e]));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float x = to_f(v[e0 + e]);
-              if (x < cut.x) continue;
-              const int q = whole(step_of(x));
+              const int q = whole(step_of(to_f(v[e0 + e])));
               atomicAdd(&S.hist[0][q], 1u);
-              if (x > cut.x) add_mass(q, w[e]);
+              if (w[e] != 0) add_mass(q, w[e]);
             }
           }
         });
-      } else {                                   // few tokens are inside the bins chosen so far
+      } else {                                   // few tokens are left by top-k, or inside the bins chosen so far
         each_vec([&](const T* v, int at) {
           uint32_t in = 0;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const float x = to_f(v[e]);
-            in |= (x >= cut.x && whole(step_of(x)) == coarse ? 1u : 0u) << e;
+            in |= (x >= cut.x && (round == 0 || whole(step_of(x)) == coarse) ? 1u : 0u) << e;
           }
           for (; in != 0; in &= in - 1) {
             const float x = to_f(vals[at + __ffs(in) - 1]);
-            if (!inside(x)) continue;
+            if (round > 0 && !inside(x)) continue;
             const int q = bin_of(x);
             atomicAdd(&S.hist[0][q], 1u);
             if (by_mass && x > cut.x) add_mass(q, weigh(x));
