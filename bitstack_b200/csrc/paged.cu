@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kTableThreads) release_pages_kernel(const uint
 // One CTA per token; a thread takes eight pairs (i, i + D/2) of a head: two 16-byte loads, two 16-byte stores, and the
 // token's cosines and sines from L1.  Bound by the copy: every byte of q, k and v is read once and written once (2047 tokens of
 // 32 / 8 heads of 128: 10.9 us, 4.5 TB/s).  The values are asked for in front of the token's position, which the table rows and
-// the destination wait for, and every thread gets the same number of items (12.6 us with 256 threads and 1.5 items each).
+// the destination wait for, and every thread gets the same number of items (12.6 us with 256 threads and 1.5 items each; two tokens per CTA 12.2).
 constexpr int kRopeThreads = 512;   // at most; the launch takes as many as give every thread the same number of items
 template <typename T>
 __global__ void __launch_bounds__(kRopeThreads) rope_paged_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,

@@ -28,8 +28,9 @@
 namespace bsb {
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kTile = 16 * kWarps;       // positions of a tile
+// Warps of a CTA; a tile is 16 positions of each.  Eight where every pair has a multiprocessor to itself: half the rounds of
+// latency of a pair (1 request of 200: 6.6 -> 5.6 us, of 512: 9.4 -> 7.9).
+constexpr int kManyWarps = 8;
 constexpr int kRows = 16;                // most query heads of one pass
 constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix sums stay in shared memory
 // What a pair costs a CTA beside its tiles, in tiles (64 ragged requests up to 8192 positions / 128 up to 1500, heads of 64: cost 0
@@ -37,8 +38,8 @@ constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix
 constexpr int kPairCost = 3;
 constexpr float kSlack = 6.f;            // see the running maximum
 // Requests that cannot be longer than this get one CTA per (request, kv head) and no join.  32 / 8 heads of 128, one CTA per pair
-// against equal shares: 1 request of 200 6.5 / 8.0 us, of 512 9.2 / 8.1, of 1000 14.6 / 8.7; 16 requests of 512 9.4 / 10.9, of 1000
-// 14.7 / 12.0; 64 requests of 200 11.2 / 15.2.
+// against equal shares: 1 request of 200 5.6 / 8.0 us, of 512 7.9 / 8.1; 16 requests of 512 7.8 / 10.9; 64 requests of 200 (four warps)
+// 11.2 / 15.2; with four warps throughout, 1 request of 1000 14.6 / 8.7, 16 of 1000 14.7 / 12.0.
 constexpr int64_t kWholePositions = 512;
 // Stages of a warp's ring, CTAs of a multiprocessor (64 ragged requests: 2 x 3 141 us, 3 x 2 147, 4 x 1 183, before the last steps).
 template <int D> struct Shape;
@@ -113,7 +114,8 @@ __device__ __forceinline__ int length_of(const AttnParams& P, int b) {
   if (pos < 0) return 0;
   return pos < P.most && pos < P.table_len ? (int)pos + 1 : -1;
 }
-__device__ __forceinline__ int tiles_of(int n) { return n <= 0 ? 1 : (n + kTile - 1) / kTile; }   // idle rows too have an output
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int n) { return n <= 0 ? 1 : (n + TILE - 1) / TILE; }   // idle rows too have an output
 
 // four values of the type as fp32; and back, leaving in x what the rounding took
 template <typename T>
@@ -159,18 +161,19 @@ __device__ __forceinline__ void turn8(const T* src, const T* cos_t, const T* sin
 }
 
 // dynamic shared memory: [warp][stage][K 16 rows, V 16 rows], q [16 rows], maxima and sums [2][warp][16], prefix sums [batch + 1]
-template <int D> constexpr int ring_bytes() { return kWarps * Shape<D>::stages * 2 * 16 * D * 2; }
-template <int D> constexpr int fixed_bytes() { return ring_bytes<D>() + 2 * kRows * D * 2 + 2 * kWarps * kRows * 4; }
+template <int D, int W> constexpr int ring_bytes() { return W * Shape<D>::stages * 2 * 16 * D * 2; }
+template <int D, int W> constexpr int fixed_bytes() { return ring_bytes<D, W>() + 2 * kRows * D * 2 + 2 * W * kRows * 4; }
 
 // NB: column blocks of 8 heads.  ALIGNED: pages are a multiple of 16 rows, so the 16 positions of a warp lie in one page.
-template <typename T, int D, int NB, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_attention_kernel(const __grid_constant__ AttnParams P) {
+template <typename T, int D, int NB, bool ALIGNED, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 1 ? Shape<D>::ctas : 2) paged_attention_kernel(const __grid_constant__ AttnParams P) {
+  constexpr int kThreads = kWarps * 32, kTile = 16 * kWarps;
   constexpr int kStages = Shape<D>::stages;
   constexpr int kChunks = D / 8;                 // 16-byte pieces of a row
   constexpr int kStep = 32 / kChunks;            // rows that one warp-wide copy covers
   constexpr int kHalf = 16 * D * 2;              // bytes of the K (or V) rows of a stage
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* s_q = smem + ring_bytes<D>();
+  uint8_t* s_q = smem + ring_bytes<D, kWarps>();
   float* s_m = reinterpret_cast<float*>(s_q + 2 * kRows * D * 2);
   float* s_l = s_m + kWarps * kRows;
   int64_t* s_before = reinterpret_cast<int64_t*>(s_l + kWarps * kRows);
@@ -189,12 +192,12 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     b = blockIdx.x / pairs;
     pair = blockIdx.x - b * pairs;
     first = 0;
-    end = tiles_of(length_of(P, b));
+    end = tiles_of<kTile>(length_of(P, b));
   } else {
     const int each = (P.batch + kThreads - 1) / kThreads;
     const int lo = min(tid * each, P.batch), hi = min(lo + each, P.batch);
     int64_t mine = 0;
-    for (int i = lo; i < hi; ++i) mine += cost + tiles_of(length_of(P, i));
+    for (int i = lo; i < hi; ++i) mine += cost + tiles_of<kTile>(length_of(P, i));
     int64_t upto = mine;
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
@@ -206,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     int64_t run = upto - mine;
     for (int i = lo; i < hi; ++i) {
       s_before[i] = run;
-      run += cost + tiles_of(length_of(P, i));
+      run += cost + tiles_of<kTile>(length_of(P, i));
     }
     if (tid == kThreads - 1) s_before[P.batch] = upto;
     __syncthreads();
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? Shape<D>::ctas : 2) paged_
     const int len = length_of(P, b);
     n = max(len, 0);
     bad = len < 0;
-    tiles = tiles_of(len);
+    tiles = tiles_of<kTile>(len);
     used = (int)min((int64_t)(tiles + cost - u0), end - at);
     t0 = max(u0 - cost, 0);
     nt = u0 + used - cost - t0;
@@ -642,24 +645,32 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   }
 }
 
-template <typename T, int D, int NB, bool ALIGNED>
-int launch_paged_attention(AttnParams P, cudaStream_t s) {
-  constexpr int kCtas = NB == 1 ? Shape<D>::ctas : 2;
-  const int pairs = P.Hkv * P.chunks;
-  P.whole = P.most <= kWholePositions;
-  const int grid = P.whole ? P.batch * pairs : sm_count() * kCtas;
-  const size_t smem = fixed_bytes<D>() + (P.whole ? 0 : (size_t)(P.batch + 1) * 8);
+template <typename T, int D, int NB, bool ALIGNED, int W>
+int launch_paged_attention(const AttnParams& P, int grid, cudaStream_t s) {
+  constexpr int kMost = fixed_bytes<D, W>() + (W == kManyWarps ? 0 : (kMaxBatch + 1) * 8);
   static bool attr_set[64] = {false};
   int dev = 0;
   BSB_CUDA(cudaGetDevice(&dev));
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, NB, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  fixed_bytes<D>() + (kMaxBatch + 1) * 8));
+    BSB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, D, NB, ALIGNED, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     attr_set[dev] = true;
   }
-  BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, NB, ALIGNED>, dim3(grid), dim3(kThreads), smem, s, P));
-  if (int rc = check_launch("paged_attention_kernel")) return rc;
-  if (P.whole) return BSB_OK;
+  const size_t smem = fixed_bytes<D, W>() + (P.whole ? 0 : (size_t)(P.batch + 1) * 8);
+  BSB_CUDA(launch_pdl(paged_attention_kernel<T, D, NB, ALIGNED, W>, dim3(grid), dim3(W * 32), smem, s, P));
+  return check_launch("paged_attention_kernel");
+}
+template <typename T, int D, int NB, bool ALIGNED>
+int launch_paged_attention(AttnParams P, cudaStream_t s) {
+  const int pairs = P.Hkv * P.chunks;
+  P.whole = P.most <= kWholePositions;
+  if (P.whole) {
+    const int grid = P.batch * pairs;
+    if constexpr (NB == 1)
+      if (grid <= sm_count()) return launch_paged_attention<T, D, NB, ALIGNED, kManyWarps>(P, grid, s);
+    return launch_paged_attention<T, D, NB, ALIGNED, 4>(P, grid, s);
+  }
+  const int grid = sm_count() * (NB == 1 ? Shape<D>::ctas : 2);
+  if (int rc = launch_paged_attention<T, D, NB, ALIGNED, 4>(P, grid, s)) return rc;
   BSB_CUDA(launch_pdl(paged_attention_join_kernel<T, D>, dim3(grid), dim3(kJoinThreads), 0, s, P));
   return check_launch("paged_attention_join_kernel");
 }
