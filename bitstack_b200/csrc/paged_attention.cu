@@ -7,7 +7,7 @@
 //    sequence, of which every CTA takes the same number.  Lengths are only known on the device, so every CTA finds its place
 //    by a prefix sum over the requests.  A pair that several CTAs share leaves partial results (maximum, sum, unnormalised
 //    output), which a second kernel joins in CTA order: no atomics, no state between calls, the same bits every time.
-//  * A CTA is four warps, and a warp is on its own: it streams its 16 positions of every tile through a ring of its own in
+//  * A CTA is four warps (eight: see kManyWarps), and a warp is on its own: it streams its 16 positions of every tile through a ring of its own in
 //    shared memory (16-byte cp.async, rows looked up page by page, so a page may end anywhere) and needs no barrier with the
 //    others until the pair ends.  Rows behind the last position are filled with zeros, whatever the page holds there.
 //  * All query heads of a group share the K and V that were read.  The products are taken transposed, scores^T = K Q^T and
