@@ -253,7 +253,7 @@ int bsb_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t batc
   int* status = device_status_word();
   if (status == nullptr) return BSB_ECUDA;
   const size_t smem = (size_t)batch * 8;
-  if (smem > 48 * 1024)
+  if (smem > 40 * 1024)                  // (48 KB without it, the kernel's static part included)
     BSB_CUDA(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTableRows * 8));
   BSB_CUDA(launch_pdl(page_tables_kernel, dim3(1), dim3(kTableThreads), smem, (cudaStream_t)stream, lens, new_tokens, batch, block_table,
                       table_stride, table_width, free_pages, free_count, capacity, page_size, max_tokens, slots, positions, offsets, last,

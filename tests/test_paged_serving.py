@@ -56,7 +56,8 @@ def _ref_tables(lens, new, table, free, count, ps, max_tokens):
 
 @pytest.mark.parametrize("batch,ps,most,grow,short,width", [
     (1, 16, 1, 1, 0, 4), (5, 1, 9, 1, 0, 40), (33, 16, 100, 1, 0, 12), (40, 24, 300, 200, 0, 40), (40, 24, 300, 200, 9, 40),
-    (64, 8, 100, 60, 30, 16), (1500, 16, 70, 1, 11, 8), (2100, 4, 20, 9, 0, 16)])
+    (64, 8, 100, 60, 30, 16), (1500, 16, 70, 1, 11, 8), (2100, 4, 20, 9, 0, 16),
+    (5120, 16, 20, 1, 0, 3), (6144, 16, 20, 1, 5, 3), (8192, 16, 20, 1, 0, 3)])
 def test_page_tables(batch, ps, most, grow, short, width):
     g = torch.Generator().manual_seed(batch * 31 + ps)
     lens = torch.randint(0, most + 1, (batch,), generator=g, dtype=torch.int32)
