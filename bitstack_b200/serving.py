@@ -78,6 +78,9 @@ class PagedDecoder:
             raise ValueError("a prompt must have at least one token")
         if max(lengths) > self.max_positions:
             raise ValueError(f"a prompt of {max(lengths)} tokens is longer than a request's {self.max_positions} positions")
+        ids = torch.cat([p.reshape(-1) for p in prompts]).to(self.device)
+        if ids.dtype not in (torch.int32, torch.int64) or bool(((ids < 0) | (ids >= self.model.shape.vocab)).any()):
+            raise ValueError(f"prompts must be integer tokens in [0, {self.model.shape.vocab})")
         free = self.free_rows()
         if len(free) < len(prompts):
             raise OutOfPages(f"{len(prompts)} prompts, {len(free)} free rows")
@@ -91,7 +94,6 @@ class PagedDecoder:
         self.temperature[at], self.top_k[at], self.top_p[at], self.min_p[at] = float(temperature), int(top_k), float(top_p), float(min_p)
         slots, positions, _, _ = glue.page_tables(self.lens, new, self.block_table, self.free_pages, self.free_count, self.page_size, total)
         try:
-            ids = torch.cat([p.reshape(-1) for p in prompts]).to(dev)
             hidden = self._prompt(ids, slots, positions, lengths)
             logits = hidden @ self.model.lm_head.t()
             u = torch.rand(len(rows), device=dev) if uniforms is None else uniforms.to(dev, torch.float32)
@@ -114,7 +116,7 @@ class PagedDecoder:
             if not self._running[r]:
                 raise ValueError(f"row {r} runs no request")
         done = torch.zeros(self.rows, dtype=torch.bool, device=self.device)
-        done[torch.tensor(list(rows), device=self.device)] = True
+        done[torch.tensor(list(rows), dtype=torch.int64, device=self.device)] = True
         glue.release_pages(done, self.lens, self.block_table, self.free_pages, self.free_count, self.page_size)
         self.active.masked_fill_(done, 0)
         for r in rows:

@@ -212,15 +212,18 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  *   rotary embedding of q and k, k and v written into the page of that position, then softmax(q.K^T / sqrt(dim)).V over
  *   positions 0 .. positions[b], grouped-query heads, fp32 softmax; out [batch][q_heads*dim].  positions[b] == -1: the row is
  *   idle, its output is 0 and nothing is written.  Pages written by one request must not be read by another in the same call.
+ *   q (rotated too) and the keys and values at positions that exist must be finite in their type, else outputs of their heads
+ *   are NaN or infinite; what pages hold behind the last position has no effect.
  *   head_dim 64 or 128.  `scratch`: bsb_paged_attention_scratch_bytes, 16-byte aligned, contents arbitrary; calls that may
  *   overlap need one each.
  * bsb_sample_step: tokens[b] drawn from softmax(logits[b] / temperature[b]) cut by, in this order,
  *   top_k (the k largest; <= 0: off), top_p (the smallest set of the largest whose weight reaches p of what top_k left;
  *   >= 1: off), min_p (weight at least min_p of the largest; <= 0: off); ties go to the lowest index and the largest always
  *   stays.  uniforms[b] in [0, 1): the token is the first in vocabulary order whose cumulative weight exceeds u times the
- *   total.  temperature <= 0 (or NaN): the first maximum.  NaN logits count as -infinity; a row without a finite logit gives
- *   token 0.  Each of temperature (1), top_k, top_p, min_p may be NULL (off).  logprobs[b] (may be NULL): log of the token's
- *   probability among those kept.  *pos += 1 (pos may be NULL).  Same inputs, same token, bit for bit.  vocab <= 262144. */
+ *   total.  temperature <= 0 (or NaN): the first maximum.  NaN logits count as -infinity; a row that its mask leaves
+ *   nothing of (no logit above -infinity) gives token 0; +infinities share everything.  Each of
+ *   temperature (1), top_k, top_p, min_p may be NULL (off).  logprobs[b] (may be NULL): log of the token's probability among
+ *   those kept.  *pos += 1 (pos may be NULL).  Same inputs, same token, bit for bit.  vocab <= 262144. */
 int bsb_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t batch, int32_t* block_table, int64_t table_stride,
                     int32_t table_width, const int32_t* free_pages, const int32_t* free_count, int32_t capacity, int32_t page_size,
                     int64_t max_tokens, int64_t* slots, int64_t* positions, int32_t* offsets, int64_t* last, int32_t* lens_out,

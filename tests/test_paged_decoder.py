@@ -140,6 +140,17 @@ def test_pool_exhaustion(model):
         d.submit(_prompts([d.max_positions + 1], 1))
 
 
+def test_prompts_outside_the_vocabulary_are_refused(model):
+    from bitstack_b200.serving import PagedDecoder
+    d = PagedDecoder(model, rows=2, num_pages=8, page_size=8)
+    for bad in (torch.tensor([5, 1000]), torch.tensor([-1]), torch.tensor([1.0, 2.0])):
+        with pytest.raises(ValueError):
+            d.submit([torch.tensor([1, 2, 3]).to(bad.dtype), bad])
+    assert int(d.free_count) == 8 and d.lens.tolist() == [0, 0] and d.free_rows() == [0, 1]
+    d.release([])                                            # nobody ends
+    assert d.submit([torch.tensor([999], dtype=torch.int32)]) == [0]
+
+
 def test_a_request_up_to_its_last_position(model):
     """128 positions in pages of 24: six whole pages, 144 positions; then the row makes no step, and nothing is NaN."""
     from bitstack_b200 import _lib
