@@ -149,6 +149,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   row_sync();   // every CTA of the row runs before another one writes into its shared memory
   pdl_wait();   // no early release: this kernel writes *pos, which the dense decode attention reads in front of its own wait
 
+  // the row's settings, asked for together and in front of its values (one after the other where they are used, each is a wait)
+  const float temp = P.temperature ? __ldg(P.temperature + b) : 1.f, mp = P.min_p ? __ldg(P.min_p + b) : 0.f, number = __ldg(P.uniforms + b);
+  float p = P.top_p ? __ldg(P.top_p + b) : 1.f;
+  int32_t k = P.top_k ? __ldg(P.top_k + b) : 0;
   // ---- the row's values and their maximum; tokens that fill up the last run are -infinity -------------------------------
   const T* row = (const T*)P.logits + b * P.stride + base;
   float top = -INFINITY;
@@ -200,7 +204,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (tid < C) cluster.map_shared_rank(&S, tid)->ex.top[rank] = top;
   row_sync();
   for (int i = 0; i < C; ++i) top = fmaxf(top, S.ex.top[i]);
-  const float temp = P.temperature ? P.temperature[b] : 1.f;
   if (b == 0 && rank == 0 && tid == 0 && P.pos != nullptr) *P.pos += 1;
   if (top == -INFINITY) {                        // a row that its mask leaves nothing of: token 0, as the greedy step gives
     if (rank == 0 && tid == 0) {
@@ -240,10 +243,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const double per_logit = fmax(1.4426950408889634074 / (double)temp, 1e-290);
   const Weigher weigh{S.powers, per_logit * 256.0, (double)top, (uint32_t)__double2hiint(-256.0 * (P.unit + 2)), P.unit};
 
-  const float mp = P.min_p ? P.min_p[b] : 0.f;
   const double least = mp > 0.f ? (double)fminf(mp, 1.f) * (double)(1ull << P.unit) : 0.0;   // the likeliest token always stays
   const uint64_t fewest = (uint64_t)ceil(least);   // units of a token that stays
-  const double u = P.uniforms[b] > 0.f ? (double)fminf(P.uniforms[b], 0.99999994f) : 0.0;
+  const double u = number > 0.f ? (double)fminf(number, 0.99999994f) : 0.0;
   auto chosen = [&](int64_t token, float x, uint64_t total) {
     P.tokens[b] = token;
     if (P.logprobs) P.logprobs[b] = (float)(((double)x - (double)top) * per_logit * 0.6931471805599453094 - log((double)total / (double)(1ull << P.unit)));
@@ -273,9 +275,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   };
 
   Cut cut{-INFINITY, 0, 0};                      // nothing is cut (tokens at -infinity have no weight)
-  int32_t k = P.top_k ? P.top_k[b] : 0;
   if (k < 0 || k >= P.vocab) k = 0;
-  float p = P.top_p ? P.top_p[b] : 1.f;
   if (p <= 0.f) {                                // the likeliest token alone
     cut = Cut{top, 1, 1};
     p = 1.f;
