@@ -12,8 +12,8 @@
 // Draw.  The first index in vocabulary order whose cumulative kept weight exceeds u times the total: weights of runs of 256
 // tokens, the run by a scan, the token inside it by one warp.
 //
-// Measured: one row of 128256 fp16 logits, top-k 50 and top-p 0.9: 14 us; 64 rows, each with settings of its own: 65 us; 256 rows of
-// 32000 fp32 logits, top-p: 77 us.  Bound by instructions (half the issue slots; the exponentials of the tokens that top-p looks
+// Measured: one row of 128256 fp16 logits, top-k 50 and top-p 0.9: 14 us; 64 rows, each with settings of its own: 62-75 us; 256 rows of
+// 32000 fp32 logits, top-p: 75 us.  Bound by instructions (half the issue slots; the exponentials of the tokens that top-p looks
 // at, three limb additions each) and, for few rows, by the barriers of the cluster.
 //
 // A row is a cluster of up to 8 CTAs, each with its part of the row in shared memory: the logits are read once, and
@@ -288,6 +288,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     Found f{0, 0, by_mass ? 0.0 : (double)k, 0, 0, 0};
     double want_all = f.want;
     mask = bits = 0;
+    // Bounds of the tokens that a pass has to look at: the cut, and from the second round on the chosen step with a margin (rounding
+    // is monotone, and a step's rounding errors stay far below 0.01); two comparisons where the step itself takes six instructions
+    // (64 rows of 128256, top-k 1000 and top-p 64 -> 59 us, each with its own settings 66 -> 64).
+    float lowest = cut.x, highest = INFINITY;
 #pragma unroll 1
     for (round = 0;; ++round) {
       if (round > 0) row_sync();                 // (every CTA has read the histograms of the round before)
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const float x = to_f(v[e]);
-            in |= (x >= cut.x && (round == 0 || whole(step_of(x)) == coarse) ? 1u : 0u) << e;
+            in |= (x >= lowest && x <= highest ? 1u : 0u) << e;
           }
           for (; in != 0; in &= in - 1) {
             const float x = to_f(vals[at + __ffs(in) - 1]);
@@ -399,8 +403,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       if (round == 0) want_all = want;
       // what is wanted of the bin; never more than it holds, whichever way 2^62 rounds
       f.want = by_mass ? fmin(want - (double)g.above_mass, (double)g.mass) : want - (double)g.above;
-      if (round == 0) coarse = g.bin;
-      else if (round == 1) fine = g.bin;
+      if (round == 0) {
+        coarse = g.bin;
+        if (coarse < kBins - 1) lowest = fmaxf(lowest, top - ((float)coarse + 0.51f) / steps);
+        highest = top - ((float)coarse - 0.51f) / steps;
+      } else if (round == 1) fine = g.bin;
       else {
         bits |= (uint32_t)(kBins - 1 - g.bin) << shift_of(round);
         mask |= 1023u << shift_of(round);
@@ -420,6 +427,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
     // The tokens of the bin into the leader's list; where all from the top on are few, those: then the leader finishes alone.
     const bool all = round == 1 && f.above + f.count <= kList;
+    if (all) highest = INFINITY;
     if (tid == 0) S.own_listed = 0;
     __syncthreads();
     each_vec([&](const T* v, int at) {
@@ -427,13 +435,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         const float x = to_f(v[e]);
-        const int q = whole(step_of(x));
-        in |= (x >= cut.x && (all ? q <= coarse : q == coarse) ? 1u : 0u) << e;
+        in |= (x >= lowest && x <= highest ? 1u : 0u) << e;
       }
       for (; in != 0; in &= in - 1) {
         const int e = __ffs(in) - 1;
         const float x = to_f(vals[at + e]);
-        if (!all && !inside(x)) continue;
+        if (all ? whole(step_of(x)) > coarse : !inside(x)) continue;
         const uint32_t i = atomicAdd(&S.own_listed, 1u);
         if (i < kList) {
           S.own_x[i] = x;
