@@ -14,9 +14,9 @@
 //    output^T = V^T P^T, so that positions and dimensions fill the 16 rows of mma.sync m16n8k16 and the heads its 8 columns: a
 //    group of up to 8 heads wastes nothing (half the MMAs, exponentials and accumulators of the untransposed form), one of up
 //    to 16 takes two column blocks.  q after its rotation and the weights go in as two values of the type each, the nearest one
-//    and what that leaves: twice the MMAs, 1 % of the time (117 -> 118 us, 64 requests), and the only rounding that is left is
-//    the output's (without: twice its error).  Scores and output are accumulated in fp32; one pass keeps the running maximum
-//    and sum.
+//    and what that leaves: twice the MMAs, 1 % of the time (117 -> 118 us, 64 requests).  Beside the output's rounding that leaves
+//    2^-22 of a value (bf16 2^-16), below fp16's normal range 2^-25 in q and 2^-38 of the largest weight (see Exponents); single
+//    values had twice the error.  Scores and output are accumulated in fp32; one pass keeps the running maximum and sum.
 //  * The new position's K and V come from the projection's output: turned, stored to the page and to the ring by the warp
 //    that meets the position, so nothing is read back.
 #include <climits>
@@ -36,7 +36,13 @@ constexpr int kMaxBatch = 2048;          // requests of one launch: their prefix
 // What a pair costs a CTA beside its tiles, in tiles (64 ragged requests up to 8192 positions / 128 up to 1500, heads of 64: cost 0
 // 143 / 37 us, 1 126 / 29.5, 3 120 / 23.3, 6 120 / 25.4).
 constexpr int kPairCost = 3;
-constexpr float kSlack = 6.f;            // see the running maximum
+// Weights are 2^(score - reference + bias), the reference being a running maximum that may fall behind by 2^slack; bias cancels in
+// the division.  fp16 holds weights from 2^-24 on only: without a bias those of a few thousand positions 17 nats below the leading
+// one vanished from the product, and not from the sum.  With 2 and 13 the largest weight lies in 2^13 .. 2^15, and what two
+// values of the type leave of a weight stays below 2^-38 of it.  bf16 has fp32's exponents.
+template <typename T> struct Exponents;
+template <> struct Exponents<__half> { static constexpr float slack = 2.f, bias = 13.f; };
+template <> struct Exponents<__nv_bfloat16> { static constexpr float slack = 6.f, bias = 0.f; };
 // Requests that cannot be longer than this get one CTA per (request, kv head) and no join.  32 / 8 heads of 128, one CTA per pair
 // against equal shares: 1 request of 200 5.6 / 8.0 us, of 512 7.9 / 8.1; 16 requests of 512 7.8 / 10.9; 64 requests of 200 (four warps)
 // 11.2 / 15.2; with four warps throughout, 1 request of 1000 14.6 / 8.7, 16 of 1000 14.7 / 12.0.
@@ -402,7 +408,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 
 
     // heads 8h + 2 t4 and + 1 of this lane: running maximum (of the raw scores) and sum; output^T, rows = dimensions
     float m[NB][2], limit[NB][2], l[NB][2], o[NB][D / 16][4];
-    const float slack = kSlack / P.scale_log2;
+    const float slack = Exponents<T>::slack / P.scale_log2;
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
       m[h][0] = m[h][1] = limit[h][0] = limit[h][1] = -INFINITY;
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 
             if (gid + 8 >= left) s[h][2] = s[h][3] = -INFINITY;
           }
         }
-        // The reference that the exponents are taken against moves only when a score has passed it by more than 2^kSlack:
+        // The reference that the exponents are taken against moves only when a score has passed it by more than the slack:
         // weights up to that are as exact in every type here, and most tiles need no reduction over the positions.
         bool moved = false;
 #pragma unroll
@@ -478,7 +484,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 
         uint32_t pf[NB][2], pr[NB][2];            // weights^T, rows = positions, columns = heads; and what their rounding left
 #pragma unroll
         for (int h = 0; h < NB; ++h) {
-          const float c0 = -m[h][0] * P.scale_log2, c1 = -m[h][1] * P.scale_log2;
+          const float c0 = fmaf(-m[h][0], P.scale_log2, Exponents<T>::bias), c1 = fmaf(-m[h][1], P.scale_log2, Exponents<T>::bias);
           s[h][0] = fast_exp2(fmaf(s[h][0], P.scale_log2, c0));
           s[h][1] = fast_exp2(fmaf(s[h][1], P.scale_log2, c1));
           s[h][2] = fast_exp2(fmaf(s[h][2], P.scale_log2, c0));
