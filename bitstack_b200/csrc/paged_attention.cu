@@ -484,11 +484,12 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 
         uint32_t pf[NB][2], pr[NB][2];            // weights^T, rows = positions, columns = heads; and what their rounding left
 #pragma unroll
         for (int h = 0; h < NB; ++h) {
-          const float c0 = fmaf(-m[h][0], P.scale_log2, Exponents<T>::bias), c1 = fmaf(-m[h][1], P.scale_log2, Exponents<T>::bias);
-          s[h][0] = fast_exp2(fmaf(s[h][0], P.scale_log2, c0));
-          s[h][1] = fast_exp2(fmaf(s[h][1], P.scale_log2, c1));
-          s[h][2] = fast_exp2(fmaf(s[h][2], P.scale_log2, c0));
-          s[h][3] = fast_exp2(fmaf(s[h][3], P.scale_log2, c1));
+          // (the difference first: the two products apart round by more than one from scores of 10^8 on)
+          const float m0 = m[h][0], m1 = m[h][1];
+          s[h][0] = fast_exp2(fmaf(s[h][0] - m0, P.scale_log2, Exponents<T>::bias));
+          s[h][1] = fast_exp2(fmaf(s[h][1] - m1, P.scale_log2, Exponents<T>::bias));
+          s[h][2] = fast_exp2(fmaf(s[h][2] - m0, P.scale_log2, Exponents<T>::bias));
+          s[h][3] = fast_exp2(fmaf(s[h][3] - m1, P.scale_log2, Exponents<T>::bias));
           l[h][0] += s[h][0] + s[h][2];
           l[h][1] += s[h][1] + s[h][3];
 #pragma unroll
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 
         for (int w = 4; w < 32; w <<= 1) l[h][e] += __shfl_xor_sync(0xFFFFFFFFu, l[h][e], w);
         const int r = h * 8 + t4 * 2 + e;
         if (gid == 0) {
-          s_m[warp * kRows + r] = m[h][e] * P.scale_log2;
+          s_m[warp * kRows + r] = m[h][e];
           s_l[warp * kRows + r] = l[h][e];
         }
         if (r < done_heads) {
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kManyWarps ? 1 : NB == 
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float mw = s_m[w * kRows + r], f = mw == -INFINITY ? 0.f : fast_exp2(mw - top);
+        const float mw = s_m[w * kRows + r], f = mw == -INFINITY ? 0.f : fast_exp2((mw - top) * P.scale_log2);
         const float4 x = *reinterpret_cast<const float4*>(smem + w * (kStages * 2 * kHalf) + (r * D + (c ^ ((r & 7) * 8))) * 4);
         sum += s_l[w * kRows + r] * f;
         a.x += x.x * f;
@@ -623,14 +624,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
         const float mi = part[r], li = part[kRows + r];
         const float4 o = *reinterpret_cast<const float4*>(part + 2 * kRows + r * D + c);
         const float top = fmaxf(m, mi);
-        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top), g = mi == -INFINITY ? 0.f : fast_exp2(mi - top);
+        const float f = m == -INFINITY ? 0.f : fast_exp2((m - top) * P.scale_log2), g = mi == -INFINITY ? 0.f : fast_exp2((mi - top) * P.scale_log2);
         m = top;
         l = l * f + li * g;
         a = make_float4(a.x * f + o.x * g, a.y * f + o.y * g, a.z * f + o.z * g, a.w * f + o.w * g);
       }
       float top = m;
       for (int w = 1; w < lanes; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
-      const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+      const float f = m == -INFINITY ? 0.f : fast_exp2((m - top) * P.scale_log2);
       l *= f;
       a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
       for (int w = 1; w < lanes; w <<= 1) {

@@ -212,8 +212,8 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  *   rotary embedding of q and k, k and v written into the page of that position, then softmax(q.K^T / sqrt(dim)).V over
  *   positions 0 .. positions[b], grouped-query heads, fp32 softmax; out [batch][q_heads*dim].  positions[b] == -1: the row is
  *   idle, its output is 0 and nothing is written.  Pages written by one request must not be read by another in the same call.
- *   q (rotated too) and the keys and values at positions that exist must be finite in their type, else outputs of their heads
- *   are NaN or infinite; what pages hold behind the last position has no effect.
+ *   q (rotated too) and the keys and values at positions that exist must be finite in their type, and q.K^T in fp32, else outputs
+ *   of their heads are NaN or infinite; what pages hold behind the last position has no effect.
  *   head_dim 64 or 128.  `scratch`: bsb_paged_attention_scratch_bytes, 16-byte aligned, contents arbitrary; calls that may
  *   overlap need one each.
  * bsb_sample_step: tokens[b] drawn from softmax(logits[b] / temperature[b]) cut by, in this order,

@@ -110,3 +110,23 @@ def test_many_small_weights_beside_a_large_one(n, lead, hkv, dtype):
     q = q.view(4, hq * d)
     out = glue.paged_decode_attention(q, k, v, cos, sin, torch.full((4,), n - 1, device=DEV), table, kp, vp, hq, hkv, d)
     _check(out, q, cos, sin, [n] * 4, table, kp, vp, hq, hkv, d, ps, dtype)
+
+
+@pytest.mark.parametrize("dtype,most", [(torch.float16, 3.0e4), (torch.bfloat16, 1.0e8)])
+@pytest.mark.parametrize("n", [300, 1500])
+def test_scores_far_beyond_one(n, dtype, most):
+    """Finite q and keys whose scores are in the thousands of millions: the two equal largest ones share everything."""
+    hq, hkv, d, ps = 6, 2, 128, 16
+    kp, vp, table, g = _requests([n], hkv, ps, d, dtype, n, 0)
+    level = torch.rand(n, device=DEV, generator=g) * 0.5 + 0.25       # of the largest: far enough below it
+    level[5] = level[n - 100] = 1.0
+    keys = (level * most)[None, :, None].expand(hkv, n, d).to(dtype)
+    _put(kp, table, 0, n, ps, keys)
+    q = (most * torch.tensor([1.0, 0.93, 0.77, 0.61, 0.53, 0.37], device=DEV))[:, None].expand(hq, d).to(dtype).reshape(1, hq * d).contiguous()
+    cos, sin = _plain_rotary(n, d, dtype)
+    v = torch.randn(1, hkv * d, device=DEV, generator=g).to(dtype)
+    out = glue.paged_decode_attention(q, keys[:, n - 1].reshape(1, hkv * d), v, cos, sin, torch.tensor([n - 1], device=DEV), table, kp, vp, hq, hkv, d)
+    values = _rows(vp, table, 0, n, ps).double()
+    want = ((values[:, 5] + values[:, n - 100]) / 2).repeat_interleave(hq // hkv, 0)
+    err = (out.view(hq, d).double() - want).abs()
+    assert bool((err <= (torch.finfo(dtype).eps / 2 + 2.0 ** -16) * want.abs() + 2.0 ** -24).all()), float(err.max())   # (NaN fails)
