@@ -82,6 +82,50 @@ def _check(out, q, cos, sin, lens, table, kp, vp, hq, hkv, d, ps, dtype):
     assert worst <= 1, worst
 
 
+_FORMS = [  # query heads, kv heads, head_dim, page size: every form of the kernel (up to 8 / more heads, pages of 16 rows or not)
+    (8, 2, 128, 16), (8, 2, 128, 24), (4, 1, 64, 16), (4, 1, 64, 7), (20, 1, 128, 32), (20, 1, 128, 24), (24, 2, 64, 64), (33, 1, 64, 9), (9, 1, 128, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d,ps", _FORMS)
+def test_random_requests(hq, hkv, d, ps, dtype):
+    """(The bound sees a lost stretch of 16 positions at all of these lengths, bf16 among them: checked on the exact weights.)"""
+    for lens, wide in (([500, 1, 0, 129, 64, 17], 0), ([1100, 63, 2049, 0, 1, 300], 40)):   # one CTA per pair; shared by CTAs
+        kp, vp, table, g = _requests(lens, hkv, ps, d, dtype, hq * 100 + ps, wide * 128 // ps)
+        q, k, v = (torch.randn(len(lens), h * d, device=DEV, generator=g).to(dtype) for h in (hq, hkv, hkv))
+        a = torch.outer(torch.arange(max(lens), device=DEV, dtype=torch.float64), 1.0 / 10000.0 ** (torch.arange(0, d, 2, device=DEV, dtype=torch.float64) / d))
+        cos, sin = (torch.cat([t, t], -1).to(dtype) for t in (a.cos(), a.sin()))
+        out = glue.paged_decode_attention(q, k, v, cos, sin, torch.tensor([n - 1 for n in lens], device=DEV), table, kp, vp, hq, hkv, d)
+        _check(out, q, cos, sin, lens, table, kp, vp, hq, hkv, d, ps, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d,ps", _FORMS)
+def test_every_stretch_of_positions_counts_once(hq, hkv, d, ps, dtype):
+    """Equal keys, and values that mark their stretch of 16 positions in a dimension of their own (every d-th shares one): a stretch
+    that is left out, taken twice or taken for another one shows in its dimension."""
+    half = torch.finfo(dtype).eps / 2
+    for lens, wide in (([512, 1, 0, 129, 64, 17, 255], 0), ([2049, 33, 0, 700, 1, 3000, 65, 1999, 128, 16], 60), ([40000], 0)):
+        kp, vp, table, _ = _requests(lens, hkv, ps, d, dtype, hq + ps, wide * 128 // ps)
+        v = torch.zeros(len(lens), hkv * d, device=DEV, dtype=dtype)
+        for b, n in enumerate(lens):
+            if n:
+                mark = torch.nn.functional.one_hot(torch.arange(n, device=DEV) // 16 % d, d).to(dtype)
+                _put(kp, table, b, n, ps, torch.zeros(hkv, n, d, device=DEV, dtype=dtype))
+                _put(vp, table, b, n, ps, mark.expand(hkv, n, d))
+                v[b] = mark[n - 1].repeat(hkv)
+        q, k = torch.randn(len(lens), hq * d, device=DEV, dtype=dtype), torch.zeros(len(lens), hkv * d, device=DEV, dtype=dtype)
+        cos, sin = _plain_rotary(max(lens), d, dtype)
+        out = glue.paged_decode_attention(q, k, v, cos, sin, torch.tensor([n - 1 for n in lens], device=DEV), table, kp, vp, hq, hkv, d)
+        for b, n in enumerate(lens):
+            want = torch.zeros(d, dtype=torch.float64, device=DEV)
+            if n:
+                want = torch.bincount(torch.arange(n, device=DEV) // 16 % d, minlength=d).double() / n
+            err = (out[b].view(hq, d).double() - want).abs()
+            # all weights are equal and exact: fp32 sums, one rounding
+            assert bool((err <= (half + 2.0 ** -16) * want + 2.0 ** -25).all()), (b, n)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("n,lead,hkv", [(400, 14.0, 1), (500, 18.0, 8), (4096, 18.0, 1), (60001, 16.0, 1), (131071, 17.5, 1), (131071, 21.0, 1),
                                         (8193, 12.0, 64), (8193, 17.5, 64), (8193, 20.0, 64)])
