@@ -140,7 +140,7 @@ def check(rc: int, what: str):
 
 def check_device_status(clear: bool = True) -> None:
     """Synchronises the current device and raises BitStackDeviceTimeout if any kernel of the library gave up a wait,
-    BitStackDeviceIndexError if one met an index outside its tensor, since the status was last cleared.  Call it wherever
-    the host waits for results anyway."""
+    BitStackDeviceIndexError if one met an index outside its tensor, since the status was last cleared (where both happened:
+    the wait, and the index at the next call).  Call it wherever the host waits for results anyway."""
     code = C.c_int32(0)
     check(load().bsb_read_status(C.byref(code), 1 if clear else 0), "device status")

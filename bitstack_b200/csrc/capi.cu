@@ -51,11 +51,12 @@ int sm_count() {
 }
 
 // ---- sticky device status -----------------------------------------------------------------------
-// One word per device, in the library image (zero when the library is loaded).  Kernels store into it only with
-// atomicCAS(word, 0, code), so the first event stays until bsb_read_status() fetches and clears it.
-static __device__ int g_status_word;
+// Two words per device, in the library image (zero when the library is loaded): waits that gave up, and indices outside their
+// tensor, so that neither hides the other.  Kernels store into them only with atomicCAS(word, 0, code), so the first event of
+// each kind stays until bsb_read_status() fetches and clears it.
+static __device__ int g_status_words[2];
 
-int* device_status_word() {
+static int* status_words() {
   static int* cached[64] = {nullptr};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
@@ -64,7 +65,7 @@ int* device_status_word() {
   }
   if (cached[dev] == nullptr) {
     void* p = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&p, g_status_word);
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_status_words);
     if (e != cudaSuccess) {
       set_error("cudaGetSymbolAddress(status word) failed: %s", cudaGetErrorString(e));
       return nullptr;
@@ -72,6 +73,11 @@ int* device_status_word() {
     cached[dev] = (int*)p;
   }
   return cached[dev];
+}
+int* device_status_word() { return status_words(); }
+int* device_index_word() {
+  int* words = status_words();
+  return words == nullptr ? nullptr : words + 1;
 }
 
 int check_weight(const bsb_weight* w) {
@@ -349,20 +355,21 @@ int64_t bsb_linear_grouped_workspace_bytes(const bsb_weight* ws, int32_t n_weigh
 
 int bsb_read_status(int32_t* code_out, int32_t clear) {
   BSB_CHECK_ARG(code_out != nullptr, "NULL argument");
-  int* word = device_status_word();
-  if (word == nullptr) return BSB_ECUDA;
-  BSB_CUDA(cudaDeviceSynchronize());   // every stream of the device: the word is shared by all of them
-  BSB_CUDA(cudaMemcpy(code_out, word, 4, cudaMemcpyDeviceToHost));
-  if (clear && *code_out != 0) BSB_CUDA(cudaMemset(word, 0, 4));
-  if (*code_out >= 61) {
-    set_error("a kernel met an index outside its tensor (code %d: 61 paged attention, 62 paged cache write, 63 token list, 64 page stack)", *code_out);
-    return BSB_EDATA;
-  }
-  if (*code_out != 0) {
+  int* words = status_words();
+  if (words == nullptr) return BSB_ECUDA;
+  int32_t codes[2] = {0, 0};
+  BSB_CUDA(cudaDeviceSynchronize());   // every stream of the device: the words are shared by all of them
+  BSB_CUDA(cudaMemcpy(codes, words, 8, cudaMemcpyDeviceToHost));
+  const int which = codes[0] != 0 ? 0 : 1;   // a wait that gave up goes first; what is not reported is not cleared
+  *code_out = codes[which];
+  if (*code_out == 0) return BSB_OK;
+  if (clear) BSB_CUDA(cudaMemset(words + which, 0, 4));
+  if (which == 0) {
     set_error("a time-bounded wait gave up on the device (code %d): the outputs of that call are NaN", *code_out);
     return BSB_ETIMEOUT;
   }
-  return BSB_OK;
+  set_error("a kernel met an index outside its tensor (code %d: 61 paged attention, 62 paged cache write, 63 token list, 64 page stack)", *code_out);
+  return BSB_EDATA;
 }
 
 int bsb_set_wait_limit_ms(int32_t ms) {
@@ -435,9 +442,11 @@ int bsb_linear_forward_host(const bsb_weight* w, const uint16_t* host_x, int64_t
     return rc;
   BSB_CUDA(cudaMemcpyAsync(host_y, dev_y, (size_t)rows * w->out_features * 2, cudaMemcpyDeviceToHost, s));
   int32_t code = 0;
-  BSB_CUDA(cudaMemcpyAsync(&code, device_status_word(), 4, cudaMemcpyDeviceToHost, s));
+  const int* word = device_status_word();
+  if (word == nullptr) return BSB_ECUDA;
+  BSB_CUDA(cudaMemcpyAsync(&code, word, 4, cudaMemcpyDeviceToHost, s));
   BSB_CUDA(cudaStreamSynchronize(s));
-  if (code != 0 && code < 61) {   // the call's outputs are NaN; the word stays set until bsb_read_status() clears it
+  if (code != 0) {   // the call's outputs are NaN; the word stays set until bsb_read_status() clears it
     set_error("a time-bounded wait gave up on the device (code %d)", code);
     return BSB_ETIMEOUT;
   }

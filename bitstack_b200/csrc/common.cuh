@@ -91,6 +91,8 @@ int check_weight(const bsb_weight* w);
 // cudaGetSymbolAddress; nullptr + error text when that fails).  A kernel whose time-bounded wait gives up stores
 // a non-zero code there with atomicCAS(word, 0, code): the first event stays until bsb_read_status() clears it.
 int* device_status_word();
+// The same for kernels that meet an index outside its tensor: a word of its own, so that neither kind hides the other.
+int* device_index_word();
 
 // ---- launchers implemented in the kernel translation units -------------------
 int launch_pack_sign(const int8_t* sign, int64_t n, uint8_t* packed, int32_t* bad, cudaStream_t s);

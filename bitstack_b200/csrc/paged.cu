@@ -250,7 +250,7 @@ int bsb_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t batc
     set_error("page tables: at most %d requests per call (got %d)", kTableRows, batch);
     return BSB_ELIMIT;
   }
-  int* status = device_status_word();
+  int* status = device_index_word();
   if (status == nullptr) return BSB_ECUDA;
   const size_t smem = (size_t)batch * 8;
   if (smem > 40 * 1024)                  // (48 KB without it, the kernel's static part included)
@@ -274,7 +274,7 @@ int bsb_release_pages(const uint8_t* done, int32_t* lens, int32_t batch, const i
     set_error("release pages: at most %d requests per call (got %d)", kTableRows, batch);
     return BSB_ELIMIT;
   }
-  int* status = device_status_word();
+  int* status = device_index_word();
   if (status == nullptr) return BSB_ECUDA;
   BSB_CUDA(launch_pdl(release_pages_kernel, dim3(1), dim3(kTableThreads), (size_t)batch * 4, (cudaStream_t)stream, done, lens, batch,
                       block_table, table_stride, table_width, free_pages, free_count, capacity, page_size, status));
@@ -298,7 +298,7 @@ int bsb_rope_paged_cache(const void* q, const void* k, const void* v, int64_t q_
   BSB_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos_table | (uintptr_t)sin_table | (uintptr_t)q_out |
                  (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0, "buffers must be 16-byte aligned");
   BSB_CHECK_ARG(tokens <= INT_MAX, "too many tokens");
-  int* status = device_status_word();
+  int* status = device_index_word();
   if (status == nullptr) return BSB_ECUDA;
   const dim3 grid((unsigned)tokens);
   const int64_t items = ((int64_t)q_heads + 2 * (int64_t)kv_heads) * (head_dim / 16), trips = ceil_div64(items, kRopeThreads);

@@ -728,7 +728,7 @@ int bsb_paged_decode_attention(const void* q, const void* k, const void* v, int6
     return BSB_EWORKSPACE;
   }
   AttnParams P;
-  P.status = device_status_word();
+  P.status = device_index_word();
   if (P.status == nullptr) return BSB_ECUDA;
   P.cos_t = cos_table;
   P.sin_t = sin_table;

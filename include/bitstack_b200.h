@@ -297,14 +297,16 @@ int bsb_linear_forward_noalloc(const bsb_weight* w, const uint16_t* x, int64_t r
  * bitstack/modules/BitStackLinear.py:103,120,152, and so must this).  Every wait inside the tcgen05 kernels is
  * time-bounded.  A wait that gives up (a hardware or driver fault, never expected in a healthy run) makes its
  * CTA write NaN to every output it was responsible for and stores a code in a per-device status word that
- * stays set until it is read -- later calls do not clear it.
- *   bsb_read_status: synchronises the current device, copies the word to *code_out and, if `clear` is non-zero,
- *     resets it.  Returns BSB_OK when the word is 0, BSB_ETIMEOUT otherwise.  Codes: 1-8 decode kernel (1 Z' ring,
- *     2 Z' slab, 3/4 operand stage full/empty, 5/6 accumulator full/empty, 7/8 sign ring), 21-24 GEMM, 31-37 fused
- *     sign-GEMM, 51 peer all-reduce.  Codes from 61 on are not waits but bad indices in device memory, and give BSB_EDATA:
- *     61 paged attention: a page outside the pool, or a position behind the table row or the cos / sin tables (the
- *     request's output is NaN); 62 bsb_rope_paged_cache: a slot outside the pool (not written) or a position behind the
- *     cos / sin tables (q row NaN, not cached); 63 bsb_page_tables: more new tokens than max_tokens (the list is cut);
+ * stays set until it is read -- later calls do not clear it.  Bad indices that kernels meet in device memory have a word of
+ * their own.
+ *   bsb_read_status: synchronises the current device, copies the code to *code_out and, if `clear` is non-zero,
+ *     resets it.  Returns BSB_OK when both words are 0, BSB_ETIMEOUT for a wait that gave up, else BSB_EDATA for a bad
+ *     index.  With both pending the wait is reported (and cleared) first, the index by the next call.
+ *     Waits: 1-8 decode kernel (1 Z' ring, 2 Z' slab, 3/4 operand stage full/empty, 5/6 accumulator full/empty, 7/8 sign
+ *     ring), 21-24 GEMM, 31-37 fused sign-GEMM, 51 peer all-reduce.
+ *     Indices: 61 paged attention: a page outside the pool, or a position behind the table row or the cos / sin tables
+ *     (the request's output is NaN); 62 bsb_rope_paged_cache: a slot outside the pool (not written) or a position behind
+ *     the cos / sin tables (q row NaN, not cached); 63 bsb_page_tables: more new tokens than max_tokens (the list is cut);
  *     64 bsb_release_pages: more pages than the stack has room for (the rest are lost).
  *     Call it wherever the host synchronises anyway (bsb_linear_forward_host does).
  *   bsb_set_wait_limit_ms: the time limit of every such wait (default 200 ms), for kernels launched afterwards. */
