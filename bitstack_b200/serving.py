@@ -188,21 +188,25 @@ class PagedDecoder:
     @torch.no_grad()
     def capture(self):
         """Captures the step in a CUDA graph, which `step` replays from then on.  No row makes a step by it: the rows are
-        idle in the runs that warm it up."""
+        idle in the runs that warm it up, and running again afterwards, also where this raises (an earlier graph then stays)."""
         kept = self.active.clone(), self.tokens.clone(), self.logprobs.clone(), self.positions.clone()
+        here, stream, logits = torch.cuda.current_stream(self.device), torch.cuda.Stream(self.device), self.logits
         self.active.zero_()
-        stream = torch.cuda.Stream(self.device)
-        stream.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.cuda.stream(stream):
-            for _ in range(2):
+        stream.wait_stream(here)
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(2):
+                    self._step()
+            here.wait_stream(stream)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
                 self._step()
-        torch.cuda.current_stream(self.device).wait_stream(stream)
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=stream):
-            self._step()
-        for t, old in zip((self.active, self.tokens, self.logprobs, self.positions), kept):
-            t.copy_(old)
-        self._graph = graph
+            self._graph, logits = graph, self.logits
+        finally:
+            self.logits = logits
+            here.wait_stream(stream)
+            for t, old in zip((self.active, self.tokens, self.logprobs, self.positions), kept):
+                t.copy_(old)
         return graph
 
     @torch.no_grad()
