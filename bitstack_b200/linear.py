@@ -24,6 +24,7 @@ reference's ablation without sign matrices) is not supported.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -64,6 +65,23 @@ def get_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     if capturing:
         ent[1] = True
     return ent[0]
+
+
+@contextlib.contextmanager
+def own_workspace(stream: torch.cuda.Stream):
+    """Inside, calls on `stream` use a scratch tensor that no other call does, before or after; yields a list that receives it at
+    the end.  For a graph capture whose replays may run beside anything else: streams come from a pool of a few handles, so
+    another capture, or eager calls, may meet the same one later.  Whoever holds the graph keeps the list."""
+    key = (stream.device.index, stream.cuda_stream)
+    others, held = _workspaces.pop(key, None), []
+    try:
+        yield held
+    finally:
+        mine = _workspaces.pop(key, None)
+        if mine is not None:
+            held.append(mine[0])
+        if others is not None:
+            _workspaces[key] = others
 
 
 @torch.no_grad()

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 
 from . import _lib, glue
 from .decode import BitStackLlamaDecoder
-from .linear import forward_grouped
+from .linear import forward_grouped, own_workspace
 
 
 class OutOfPages(RuntimeError):
@@ -194,13 +194,15 @@ class PagedDecoder:
         self.active.zero_()
         stream.wait_stream(here)
         try:
-            with torch.cuda.stream(stream):
-                for _ in range(2):
+            with own_workspace(stream) as scratch:
+                with torch.cuda.stream(stream):
+                    for _ in range(2):
+                        self._step()
+                here.wait_stream(stream)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=stream):
                     self._step()
-            here.wait_stream(stream)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, stream=stream):
-                self._step()
+            graph.scratch = scratch                            # of the projections: the graph's alone, and there as long as it is
             self._graph, logits = graph, self.logits
         finally:
             self.logits = logits

@@ -51,3 +51,41 @@ def test_a_capture_that_fails_leaves_the_requests_running(model, monkeypatch, fa
         d.capture()                                           # and a later one succeeds
         runs[-1] += [d.step().tolist() + d.positions.tolist() for _ in range(3)]
     assert runs[0] == runs[1] and all(r[3:5] == [11 + 1 + i, 30 + 1 + i] for i, r in enumerate(runs[0]))
+
+
+def test_captured_steps_share_no_scratch(model, monkeypatch):
+    """Two decoders whose captures meet the same stream handle (handles come from a small pool), and eager calls on it: each uses
+    scratch of its own, so their replays may run side by side."""
+    from bitstack_b200 import linear
+    from bitstack_b200.serving import PagedDecoder
+    stream, used, real = torch.cuda.Stream(), {}, linear.get_workspace
+
+    def spy(device, nbytes):
+        t = real(device, nbytes)
+        used.setdefault(who + (" captured" if torch.cuda.is_current_stream_capturing() else " eager"), set()).add(t.data_ptr())
+        return t
+    monkeypatch.setattr(linear, "get_workspace", spy)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda *a, **k: stream)
+    who = "before"
+    decoders = []
+    with torch.cuda.stream(stream):
+        first = PagedDecoder(model, rows=3, num_pages=20, page_size=8)
+        first.generate(_prompts([9, 5], 2), steps=3)
+    stream.synchronize()
+    for who in ("a", "b"):
+        d = PagedDecoder(model, rows=3, num_pages=20, page_size=8)
+        d.capture()
+        decoders.append(d)
+    who = "after"
+    with torch.cuda.stream(stream):
+        first.generate(_prompts([9, 5], 2), steps=3)
+    stream.synchronize()
+    a, b = used["a captured"], used["b captured"]
+    assert a and b and not a & b and not (a | b) & (used["before eager"] | used["after eager"])
+    assert used["before eager"] == used["after eager"]        # the calls outside keep theirs
+    assert [{t.data_ptr() for t in d._graph.scratch} for d in decoders] == [a, b]
+    runs = []
+    for d in decoders:
+        rows = d.submit(_prompts([9, 5], 2))
+        runs.append([d.tokens[rows].tolist()] + [d.step()[rows].tolist() for _ in range(2)])
+    assert runs[0] == runs[1] and [list(t) for t in zip(*runs[0])] == first.generate(_prompts([9, 5], 2), steps=3)
