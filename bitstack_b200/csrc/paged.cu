@@ -51,16 +51,16 @@ __device__ __forceinline__ int row_of(const int32_t* start, int n, int64_t x) {
   return lo;
 }
 
-// the slot and position of token t of the list: its request is found from the offsets, its position counts back from the
-// request's last one, its page is in the table
-__device__ __forceinline__ void token_entry(int64_t t, const int32_t* offsets, int batch, const int64_t* last, const int32_t* table,
-                                            int64_t table_stride, int page_size, int64_t* slots, int64_t* positions) {
+// the slot and position of token t of the list: its request is found from the offsets, its position counts from the request's
+// first new one (the offset behind the request may have been held at 2^31 - 1), its page is in the table
+__device__ __forceinline__ void token_entry(int64_t t, const int32_t* offsets, int batch, const int32_t* new_tokens, const int64_t* last,
+                                            const int32_t* table, int64_t table_stride, int page_size, int64_t* slots, int64_t* positions) {
   int64_t slot = -1, pos = -1;
   if (t < offsets[batch]) {
     const int row = row_of(offsets, batch, t);
     const int64_t end = last[row];
     if (end >= 0) {
-      pos = end - (offsets[row + 1] - 1 - t);
+      pos = end + 1 - new_tokens[row] + (t - offsets[row]);
       const int page = table[row * table_stride + (int)pos / page_size];
       slot = page < 0 ? -1 : (int64_t)page * page_size + (int)pos % page_size;
     }
@@ -127,15 +127,16 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(
   if (max_tokens > kTokensInOne) return;
   __syncthreads();
   for (int64_t t = threadIdx.x; t < max_tokens; t += kTableThreads)
-    token_entry(t, offsets, batch, last, table, table_stride, page_size, slots, positions);
+    token_entry(t, offsets, batch, new_tokens, last, table, table_stride, page_size, slots, positions);
 }
 
-__global__ void __launch_bounds__(256) page_tokens_kernel(const int32_t* __restrict__ offsets, int batch, const int64_t* __restrict__ last,
-                                                          const int32_t* __restrict__ table, int64_t table_stride, int page_size,
-                                                          int64_t max_tokens, int64_t* __restrict__ slots, int64_t* __restrict__ positions) {
+__global__ void __launch_bounds__(256) page_tokens_kernel(const int32_t* __restrict__ offsets, int batch, const int32_t* __restrict__ new_tokens,
+                                                          const int64_t* __restrict__ last, const int32_t* __restrict__ table,
+                                                          int64_t table_stride, int page_size, int64_t max_tokens,
+                                                          int64_t* __restrict__ slots, int64_t* __restrict__ positions) {
   pdl_wait();
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (t < max_tokens) token_entry(t, offsets, batch, last, table, table_stride, page_size, slots, positions);
+  if (t < max_tokens) token_entry(t, offsets, batch, new_tokens, last, table, table_stride, page_size, slots, positions);
 }
 
 // pages of the requests that are done go back on the stack, in the order of the requests and of their pages
@@ -261,8 +262,8 @@ int bsb_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t batc
   if (int rc = check_launch("page_tables_kernel")) return rc;
   if (max_tokens <= kTokensInOne) return BSB_OK;
   BSB_CUDA(launch_pdl(page_tokens_kernel, dim3((unsigned)ceil_div64(max_tokens, 256)), dim3(256), 0, (cudaStream_t)stream,
-                      (const int32_t*)offsets, batch, (const int64_t*)last, (const int32_t*)block_table, table_stride, page_size, max_tokens,
-                      slots, positions));
+                      (const int32_t*)offsets, batch, new_tokens, (const int64_t*)last, (const int32_t*)block_table, table_stride, page_size,
+                      max_tokens, slots, positions));
   return check_launch("page_tokens_kernel");
 }
 

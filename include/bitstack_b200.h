@@ -199,7 +199,8 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  *   order, and entered in its row; entries of a row behind its pages are left as they are.  A request is REFUSED when its
  *   row is too narrow, or when it needs pages and the stack holds fewer than it and the requests before it need together;
  *   it keeps its length and its place in the token list.
- *     offsets [batch + 1]       first token of every request in the list of all new tokens (request after request)
+ *     offsets [batch + 1]       first token of every request in the list of all new tokens (request after request), at most
+ *                               2^31 - 1
  *     slots, positions [max_tokens]   of every new token; -1 for tokens of a refused request and behind the list's end
  *     last [batch]              position of the request's last new token; -1 when it has none or was refused
  *     lens_out, free_count_out  lengths and stack height afterwards; may be lens and free_count themselves
