@@ -213,8 +213,10 @@ class PagedDecoder:
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[torch.Tensor], steps: int, **sampling) -> List[List[int]]:
-        """Host-facing: admits the prompts, makes `steps` tokens for each (the first of them from the prompt) and releases
-        them.  Raises OutOfPages when the pool runs out on the way."""
+        """Host-facing: admits the prompts, makes `steps` tokens (at least one) for each (the first of them from the prompt) and
+        releases them.  Raises OutOfPages when the pool runs out on the way."""
+        if steps < 1:
+            raise ValueError(f"steps must be at least 1, got {steps}: a prompt gives its first token when it is admitted")
         rows = self.submit(prompts, **sampling)
         try:
             out = [self.tokens[rows].tolist()]
