@@ -114,7 +114,8 @@ def page_tables(lens, new_tokens, block_table, free_pages, free_count, page_size
 
 
 def release_pages(done, lens, block_table, free_pages, free_count, page_size: int) -> None:
-    """Requests with done[b] (bool [batch]) give their pages back to the stack, and their length becomes 0 (in place)."""
+    """Requests with done[b] (bool [batch]) give their pages back to the stack, and their length becomes 0 (in place).  A page
+    that several rows list goes back once for each of them: rows that share pages are released with their own pages alone."""
     _lib.serving().release_pages(done, lens, block_table, free_pages, free_count, page_size)
 
 

@@ -191,8 +191,11 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  * position p of the request being row p % page_size of page block_table[b][p / page_size].  A SLOT is
  * page * page_size + row.  fp16 or bf16 (`dtype`: q, k, v, the cos / sin tables [table_len][head_dim], pages and output
  * alike), rows of q, k, v q_stride / k_stride / v_stride elements apart (multiples of 8), 16-byte aligned buffers.
- * An index that points outside its tensor is never followed: see bsb_read_status, codes 61-64.  None of these calls lets the
- * kernel behind it start before what it writes is there, so any other call may follow directly (bsb_decode_attention too).
+ * An index that points outside its tensor is never followed: see bsb_read_status, codes 61-64.  When the kernel behind one of
+ * these calls starts, the pages, tables, lengths, lists, positions and tokens that the call wrote are there; `out` of
+ * bsb_paged_decode_attention is there once that kernel has waited for the ones in front of it, as all of this library's and
+ * every ordinary launch do.  So any other call may follow directly (bsb_decode_attention too, which reads its position and
+ * older cache rows in front of that wait).
  *
  * bsb_page_tables: one step of all requests.  Request b holds lens[b] tokens and gets new_tokens[b] more (negative counts
  *   are taken as 0).  Pages it lacks are popped from the stack free_pages[0 .. *free_count) (capacity entries), requests in
@@ -205,7 +208,10 @@ int bsb_silu_mul(const uint16_t* gate, const uint16_t* up, uint16_t* out, float*
  *     last [batch]              position of the request's last new token; -1 when it has none or was refused
  *     lens_out, free_count_out  lengths and stack height afterwards; may be lens and free_count themselves
  *   max_tokens == 0: no list is written (slots and positions may be NULL).  At most 8192 requests.
- * bsb_release_pages: requests with done[b] != 0 give their pages back to the stack (in order) and get length 0.
+ * bsb_release_pages: requests with done[b] != 0 give their pages back to the stack (in order) and get length 0.  Nothing counts
+ *   how many rows list a page: one that several rows share (a common prefix) goes on the stack once for each of them that is
+ *   released, and is then handed out more than once.  The caller counts such pages: it releases a row that lists only the
+ *   pages that nobody else uses, with the length that they hold.
  * bsb_rope_paged_cache: rotary embedding ("rotate half") of `tokens` tokens: q_out [tokens][q_heads*head_dim] = rotated q;
  *   rotated k and v go to the token's slot.  Slot -1: not cached; position -1: padding, its q_out row is 0 and nothing is
  *   cached.  Slots of one call must differ.  head_dim % 16 == 0, <= 512.
