@@ -15,12 +15,10 @@ template <typename T> struct Pair;
 template <> struct Pair<__half> {
   using type = __half2;
   static __device__ __forceinline__ __half2 make(float a, float b) { return __floats2half2_rn(a, b); }
-  static __device__ __forceinline__ __half one(float a) { return __float2half_rn(a); }
 };
 template <> struct Pair<__nv_bfloat16> {
   using type = __nv_bfloat162;
   static __device__ __forceinline__ __nv_bfloat162 make(float a, float b) { return __floats2bfloat162_rn(a, b); }
-  static __device__ __forceinline__ __nv_bfloat16 one(float a) { return __float2bfloat16_rn(a); }
 };
 
 template <typename T>
