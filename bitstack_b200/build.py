@@ -9,6 +9,7 @@ calling the library through its C ABI.
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -72,9 +73,13 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None, lib_path
 
 
 def build_serving(force: bool = False, verbose: bool = False) -> str:
-    """The tensor front end (host code): g++ against the headers of the torch that this interpreter imports."""
+    """The tensor front end (host code): g++ against the headers of the torch that this interpreter imports.  It fits that torch
+    and that interpreter alone, so it is built again when either has changed."""
     src = os.path.join(CSRC, "serving_torch.cpp")
-    if not force and not _stale(SERVING_LIB, [src, HEADERS[-1]]):
+    made_for = os.path.join(HERE, "build", "serving_versions.txt")
+    versions = f"{sysconfig.get_config_var('SOABI')} torch {importlib.metadata.version('torch')}\n"
+    same = os.path.exists(made_for) and open(made_for).read() == versions
+    if not force and same and not _stale(SERVING_LIB, [src, HEADERS[-1]]):
         return SERVING_LIB
     spec = importlib.util.find_spec("torch")
     if spec is None:
@@ -89,6 +94,9 @@ def build_serving(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         sys.stderr.write(" ".join(cmd) + "\n")
     subprocess.check_call(cmd)
+    os.makedirs(os.path.dirname(made_for), exist_ok=True)
+    with open(made_for, "w") as f:
+        f.write(versions)
     return SERVING_LIB
 
 
