@@ -56,6 +56,15 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 }
 __device__ __forceinline__ float of_order_bits(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
+// S of the weights' unit 2^-S: vocab * 2^S <= 2^62.  The sums of all weights have to stay there: past 2^64 they are no longer
+// ordered, the CTAs of a row take different ways, and one may leave while the others still read its shared memory.
+constexpr int unit_of(int64_t vocab) {
+  int s = 50;
+  while (vocab > (1ll << (62 - s))) --s;         // (vocab << s would itself pass 64 bits)
+  return s;
+}
+static_assert(unit_of(1) == 50 && unit_of(4096) == 50 && unit_of(4097) == 49 && unit_of(128256) == 45 && unit_of(kMaxVocab) == 44, "");
+
 struct Weigher {
   const double* powers;   // 2^(i/256)
   double c256, top;       // exponent in 256ths: (x - top) c256, c256 = 256 log2(e) / T
@@ -761,8 +770,7 @@ int bsb_sample_step(const void* logits, int64_t batch, int64_t vocab, int64_t ro
   P.tokens = tokens;
   P.pos = pos;
   P.logprobs = logprobs;
-  P.unit = 50;                                          // vocab * 2^unit <= 2^62
-  while ((vocab << P.unit) > (1ll << 62)) --P.unit;
+  P.unit = unit_of(vocab);
   if (dtype == BSB_F16) return launch_sample<__half>(P, batch, (cudaStream_t)stream);
   if (dtype == BSB_BF16) return launch_sample<__nv_bfloat16>(P, batch, (cudaStream_t)stream);
   return launch_sample<float>(P, batch, (cudaStream_t)stream);
