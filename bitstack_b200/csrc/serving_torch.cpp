@@ -97,7 +97,7 @@ py::tuple page_tables(const Tensor& lens, const Tensor& new_tokens, const Tensor
   need(new_tokens, "new_tokens", at::kInt, {l.batch}, l.index);
   if (lens_out) need(*lens_out, "lens_out", at::kInt, {l.batch}, l.index);
   if (free_count_out) need(*free_count_out, "free_count_out", at::kInt, {1}, l.index);
-  if (max_tokens < 0) refuse("max_tokens must not be negative");
+  small(max_tokens, "max_tokens");       // (in front of the lists' allocation)
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)l.index);
   const auto longs = lens.options().dtype(at::kLong);
   Tensor slots = at::empty({max_tokens}, longs), positions = at::empty({max_tokens}, longs), last = at::empty({l.batch}, longs);

@@ -42,3 +42,12 @@ def test_positions_of_a_list_longer_than_31_bits(lens, new, listed):
     assert total > listed
     with pytest.raises(_lib.BitStackDeviceIndexError):  # the list was cut
         _lib.check_device_status()
+
+
+@pytest.mark.parametrize("listed", [2 ** 31, 2 ** 62, -1])
+def test_lists_beyond_31_bits_are_refused_before_they_are_allocated(listed):
+    free = torch.cuda.memory_reserved()
+    lens = _i(1, 2)
+    with pytest.raises(ValueError, match="max_tokens"):
+        glue.page_tables(lens, _i(1, 1), torch.zeros(2, 3, dtype=torch.int32, device=DEV), _i(1), _i(1), 4, listed)
+    assert torch.cuda.memory_reserved() - free < 1 << 22 and lens.tolist() == [1, 2]
