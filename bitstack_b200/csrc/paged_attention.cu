@@ -2,7 +2,9 @@
 // page, softmax(q K^T / sqrt(D)) V over the request's pages.
 //
 // Bound by reading K and V once (4 flops per byte and head of a group; the floor is their bytes at copy bandwidth).  Measured: 64
-// requests of 1 to 8192 positions, 32 / 8 heads of 128: 120 us, 6.0 TB/s (copy 6.55); one request of 131071: 90 us, 6.0 TB/s.
+// requests of 1 to 8192 positions, 32 / 8 heads of 128: 121 us, 5.9 TB/s (copy 6.55); one request of 131071: 91 us, 5.9 TB/s.  The
+// prefix sums take shared memory: from about 310 requests on, heads of 64 keep three CTAs of a multiprocessor instead of
+// four (300 requests of 1500, 16 / 4 heads: 5.6 TB/s, 320: 4.6); heads of 128 do not notice (5.7 TB/s on both sides).
 //  * Work split: a request's length is cut into tiles of 64 positions; the tiles of all (request, kv head) pairs form one
 //    sequence, of which every CTA takes the same number.  Lengths are only known on the device, so every CTA finds its place
 //    by a prefix sum over the requests.  A pair that several CTAs share leaves partial results (maximum, sum, unnormalised
@@ -43,7 +45,9 @@ constexpr int kPairCost = 3;
 template <typename T> struct Exponents;
 template <> struct Exponents<__half> { static constexpr float slack = 2.f, bias = 13.f; };
 template <> struct Exponents<__nv_bfloat16> { static constexpr float slack = 6.f, bias = 0.f; };
-// Requests that cannot be longer than this get one CTA per (request, kv head) and no join.  32 / 8 heads of 128, one CTA per pair
+// Requests that cannot be longer than this by the width of their table get one CTA per (request, kv head) and no join (short ones
+// in a wide table take the shared form: 1 request of 200 8.1 us instead of 5.8, 16 up to 384 with 64 / 8 heads 12.3 instead of
+// 7.4).  32 / 8 heads of 128, one CTA per pair
 // against equal shares: 1 request of 200 5.6 / 8.0 us, of 512 7.9 / 8.1; 16 requests of 512 7.8 / 10.9; 64 requests of 200 (four warps)
 // 11.2 / 15.2; with four warps throughout, 1 request of 1000 14.6 / 8.7, 16 of 1000 14.7 / 12.0.
 constexpr int64_t kWholePositions = 512;

@@ -12,9 +12,11 @@
 // Draw.  The first index in vocabulary order whose cumulative kept weight exceeds u times the total: weights of runs of 256
 // tokens, the run by a scan, the token inside it by one warp.
 //
-// Measured: one row of 128256 fp16 logits, top-k 50 and top-p 0.9: 14 us; 64 rows, each with settings of its own: 62-75 us; 256 rows of
-// 32000 fp32 logits, top-p: 75 us.  Bound by instructions (half the issue slots; the exponentials of the tokens that top-p looks
-// at, three limb additions each) and, for few rows, by the barriers of the cluster.
+// Measured: one row of 128256 fp16 logits, top-k 50 and top-p 0.9: 14 us; 64 rows, each with settings of its own: 51-76 us, by how many
+// have a wide top-p; all with top-p 0.9 at temperature 1: 86 us; 256 rows of 32000 fp32 logits, top-p: 76 us.  Bound by the
+// instructions on the tokens that top-p looks at (their exponentials, three limb additions each in shared memory) and by barriers,
+// for few rows those of the cluster; 64 registers, with 172-204 bytes of spills.  bf16 logits of a wide top-p take 125 us where
+// fp16 ones take 86: more than kList tokens share the border's value, which is then taken apart by its bits to the last.
 //
 // A row is a cluster of up to 8 CTAs, each with its part of the row in shared memory: the logits are read once, and
 // histograms, totals and results are exchanged through distributed shared memory.
@@ -709,8 +711,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 template <typename T>
 int launch_sample(SampleParams P, int64_t batch, cudaStream_t s) {
   // CTAs of a row: enough that two parts fit a multiprocessor side by side, and more while all rows still run at once and a
-  // CTA keeps 2048 tokens (one row of 128256: 8 CTAs 17 us, 2 CTAs 19; 64 rows: 4 CTAs 70 us, 8 CTAs 82; 256 rows of 32000
-  // fp32 logits: 2 CTAs 84 us, 1 CTA 97, 4 CTAs 121)
+  // CTA keeps 2048 tokens (one row of 128256: 8 CTAs 13.9 us, 4 CTAs 15.5; 64 rows, top-p: 4 CTAs 80 us, 8 CTAs 125; 32000 fp32
+  // logits, 64 rows: 1 CTA 42 us, 2 CTAs 33, 4 CTAs 35, 8 CTAs 76; 256 rows: 1 or 2 CTAs 76 us, 4 CTAs 109)
   int cluster = 1;
   while (cluster < kMaxCluster && (P.vocab > (int64_t)kMaxPart * cluster || P.vocab * (int64_t)sizeof(T) > 80 * 1024 * cluster)) cluster *= 2;
   while (cluster < kMaxCluster && P.vocab > 2048 * cluster && batch * cluster <= sm_count()) cluster *= 2;
